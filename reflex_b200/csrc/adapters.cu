@@ -1,0 +1,290 @@
+// Adapters of a step's requests: the rows grouped by adapter, and the low-rank products in 32-bit
+// multiply-adds.
+//
+//  * rows: a stable counting sort of the rows by their adapter's number, rows without one last, and the
+//    groups cut into tiles of at most T rows.  One block: every warp counts a piece of the rows, lanes with
+//    the same number found by a match, so that nothing depends on the order of atomics; a prefix over
+//    (number, warp) gives each warp the place at which its rows of a number go.  Latency bounds it.
+//  * add: out[r, c] = base[r, c] + s_a sum_i B_a[c, i] (sum_k A_a[part(c), i, k] x[r, k]), a the row's
+//    adapter, in two launches: the low-rank rows v = A x (k in LOW_SPLITS pieces that depend on K alone, an
+//    element's products added in k's order, the pieces' sums in order, so that a row's bits do not depend on
+//    what else is in the step), then out.  Any sizes, strides and alignment, 32-bit and bfloat16.
+#include "adapters.cuh"
+
+namespace {
+
+using namespace rfx;
+using namespace adapters;
+
+constexpr int GROUP_THREADS = 1024;
+constexpr int MAX_ADAPTERS = 1024;
+
+__device__ __forceinline__ int warp_inclusive(int v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// Exclusive prefix over the block of a value a thread; `total` is the sum.  `scratch` holds 33 ints.
+__device__ __forceinline__ int block_exclusive(int v, int* scratch, int* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int in = warp_inclusive(v);
+    __syncthreads();
+    if (lane == 31) scratch[warp] = in;
+    __syncthreads();
+    if (warp == 0) {
+        const int w = scratch[lane];
+        const int s = warp_inclusive(w);
+        scratch[lane] = s - w;
+        if (lane == 31) scratch[32] = s;
+    }
+    __syncthreads();
+    *total = scratch[32];
+    return scratch[warp] + in - v;
+}
+
+// cnt[w][key]: rows of a key in warp w's piece, then the place of the first of them; two more rows: the
+// first place of every key, and the first tile of every key.
+__global__ void __launch_bounds__(GROUP_THREADS)
+adapter_rows_kernel(const int* __restrict__ ids, int R, int n, int T, int* __restrict__ order, int* __restrict__ first,
+                    int* __restrict__ tiles, int max_tiles, int* __restrict__ err) {
+    extern __shared__ int sh[];
+    __shared__ int scratch[33];
+    pdl_prologue();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = GROUP_THREADS / 32;
+    const int keys = n + 1;
+    int* cnt = sh;
+    int* s_first = sh + warps * keys;
+    int* s_tile = s_first + keys + 1;
+    const int piece = ((R + warps - 1) / warps + 31) / 32 * 32;
+    const int lo = min(R, warp * piece), hi = min(R, lo + piece);
+    for (int i = threadIdx.x; i < warps * keys; i += GROUP_THREADS) cnt[i] = 0;
+    __syncthreads();
+    int* mine = cnt + warp * keys;
+    bool bad = false;
+    auto key_of = [&](int r) {
+        if (r >= hi) return -1;
+        const int id = ids[r];
+        bad |= id < -1 || id >= n;
+        return id < 0 || id >= n ? n : id;
+    };
+    for (int r0 = lo; r0 < hi; r0 += 32) {
+        const int key = key_of(r0 + lane);
+        const unsigned same = __match_any_sync(0xffffffffu, key);
+        if (key >= 0 && lane == __ffs(same) - 1) mine[key] += __popc(same);
+        __syncwarp();
+    }
+    if (bad) atomicExch(err, 2);
+    __syncthreads();
+    // a key's count over the warps, the keys' first places and first tiles, a block's threads at a time
+    int placed = 0, tiled = 0;
+    for (int k0 = 0; k0 < keys; k0 += GROUP_THREADS) {
+        const int k = k0 + threadIdx.x;
+        int total = 0;
+        if (k < keys)
+            for (int w = 0; w < warps; ++w) {
+                const int c = cnt[w * keys + k];
+                cnt[w * keys + k] = total;
+                total += c;
+            }
+        int all, all_tiles;
+        const int at = placed + block_exclusive(total, scratch, &all);
+        const int tile = tiled + block_exclusive((total + T - 1) / T, scratch, &all_tiles);
+        if (k < keys) {
+            s_first[k] = at;
+            s_tile[k] = tile;
+            first[k] = at;
+        }
+        placed += all;
+        tiled += all_tiles;
+    }
+    if (threadIdx.x == 0) {
+        s_first[keys] = placed;
+        s_tile[keys] = tiled;
+        first[keys] = placed;
+    }
+    __syncthreads();
+    for (int r0 = lo; r0 < hi; r0 += 32) {
+        const int key = key_of(r0 + lane);
+        const unsigned same = __match_any_sync(0xffffffffu, key);
+        if (key >= 0) order[s_first[key] + mine[key] + __popc(same & ((1u << lane) - 1))] = r0 + lane;
+        __syncwarp();
+        if (key >= 0 && lane == __ffs(same) - 1) mine[key] += __popc(same);
+        __syncwarp();
+    }
+    for (int t = threadIdx.x; t < max_tiles; t += GROUP_THREADS) {
+        int a = -1, place = 0, count = 0;
+        if (t < tiled) {
+            int l = 0, h = keys - 1;  // the last key whose first tile is at or before t and that has rows
+            while (l < h) {
+                const int m = (l + h + 1) / 2;
+                if (s_tile[m] <= t) l = m;
+                else h = m - 1;
+            }
+            a = l;
+            place = s_first[l] + (t - s_tile[l]) * T;
+            count = min(T, s_first[l + 1] - place);
+        }
+        tiles[3 * t] = a;
+        tiles[3 * t + 1] = place;
+        tiles[3 * t + 2] = count;
+    }
+}
+
+// ---- the products in 32-bit multiply-adds ------------------------------------------------------------
+constexpr int LOW_SPLITS = 8, ROWS = 32, COLS = 32, BK = 32, OUT_COLS = 64;
+
+__host__ __device__ inline int k_piece(int K) { return ((K + LOW_SPLITS - 1) / LOW_SPLITS + BK - 1) / BK * BK; }
+__host__ __device__ inline int k_pieces(int K) { return (K + k_piece(K) - 1) / k_piece(K); }
+
+// low[piece][place][part * rank + i]: 32 rows x 32 rank rows a block, four sums a thread
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_low_kernel(const Args p) {
+    __shared__ float xs[ROWS][BK + 1], as[COLS][BK + 1];
+    __shared__ int rows[ROWS];
+    pdl_prologue();
+    const int subs = (p.tile + ROWS - 1) / ROWS;
+    const Tile t = load_tile(p.tiles, blockIdx.x / subs);
+    const int sub = blockIdx.x % subs * ROWS, W = p.parts.n * p.rank;
+    if (t.adapter < 0 || t.adapter >= p.n || sub >= t.count) return;
+    const int here = min(ROWS, t.count - sub), w0 = blockIdx.y * COLS, rank = p.rank_of(t.adapter);
+    const int k0 = blockIdx.z * k_piece(p.K), k1 = min(p.K, k0 + k_piece(p.K));
+    if (threadIdx.x < ROWS) rows[threadIdx.x] = p.order[t.place + sub + min((int)threadIdx.x, here - 1)];
+    __syncthreads();
+    const T* x = (const T*)p.x;
+    const T* a = (const T*)p.a + (size_t)t.adapter * W * p.lda;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = k0; k < k1; k += BK) {
+        const bool in = k + tx < k1;
+#pragma unroll
+        for (int i = ty; i < ROWS; i += 8) xs[i][tx] = in && i < here ? ld(x, (size_t)rows[i] * p.ld_x + k + tx) : 0.f;
+#pragma unroll
+        for (int i = ty; i < COLS; i += 8)
+            as[i][tx] = in && w0 + i < W && (w0 + i) % p.rank < rank ? ld(a, (size_t)(w0 + i) * p.lda + k + tx) : 0.f;
+        __syncthreads();
+        const int most = min(BK, k1 - k);
+        for (int kk = 0; kk < most; ++kk)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = fmaf(xs[ty * 4 + j][kk], as[tx][kk], acc[j]);
+        __syncthreads();
+    }
+    if (w0 + tx < W)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (ty * 4 + j < here)
+                p.low[((size_t)blockIdx.z * p.R + t.place + sub + ty * 4 + j) * W + w0 + tx] = acc[j];
+}
+
+// 32 rows x 64 columns a block, eight rows a thread
+template <typename T, typename TO>
+__global__ void __launch_bounds__(256) adapter_up_kernel(const Args p) {
+    extern __shared__ float vs[];  // [ROWS][W]
+    __shared__ int rows[ROWS];
+    pdl_prologue();
+    const int subs = (p.tile + ROWS - 1) / ROWS;
+    const Tile t = load_tile(p.tiles, blockIdx.x / subs);
+    const int sub = blockIdx.x % subs * ROWS, W = p.parts.n * p.rank;
+    if (t.adapter < 0 || sub >= t.count) return;
+    const bool none = t.adapter >= p.n;
+    if (none && p.out == p.base) return;
+    const int here = min(ROWS, t.count - sub);
+    if (threadIdx.x < ROWS) rows[threadIdx.x] = p.order[t.place + sub + min((int)threadIdx.x, here - 1)];
+    const int pieces = k_pieces(p.K);
+    if (!none)
+        for (int i = threadIdx.x; i < here * W; i += 256) {
+            float v = 0.f;
+            for (int s = 0; s < pieces; ++s) v += p.low[((size_t)s * p.R + t.place + sub) * W + i];
+            vs[i] = v;
+        }
+    __syncthreads();
+    const int c = blockIdx.y * OUT_COLS + (threadIdx.x & 63), r0 = (threadIdx.x >> 6) * 8;
+    if (c >= p.N) return;
+    const TO* base = (const TO*)p.base;
+    TO* out = (TO*)p.out;
+    float acc[8] = {};
+    float scale = 0.f;
+    if (!none) {
+        const int rank = p.rank_of(t.adapter);
+        const T* b = (const T*)p.b + ((size_t)t.adapter * p.N + c) * p.rank;
+        const float* v = vs + p.parts.part_of(c) * p.rank;
+        scale = p.scale[t.adapter];
+        for (int i = 0; i < rank; ++i) {
+            const float bi = ld(b, i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (r0 + j < here) acc[j] = fmaf(v[(r0 + j) * W + i], bi, acc[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (r0 + j < here) {
+            const float y = ld(base, (size_t)rows[r0 + j] * p.ld_base + c);
+            st(out, (size_t)rows[r0 + j] * p.ld_out + c, none ? y : fmaf(scale, acc[j], y));
+        }
+}
+
+template <typename T, typename TO>
+int fma_form(const Args& p, cudaStream_t s) {
+    const int W = p.parts.n * p.rank, subs = (p.tile + ROWS - 1) / ROWS;
+    const long long blocks = (long long)p.max_tiles * subs;
+    if (blocks > 0x7fffffffLL || (p.N + OUT_COLS - 1) / OUT_COLS > 65535 || (W + COLS - 1) / COLS > 65535)
+        return RFX_ERR_UNSUPPORTED;
+    const size_t smem = (size_t)ROWS * W * sizeof(float);
+    cudaError_t e = cudaFuncSetAttribute(adapter_up_kernel<T, TO>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    RFX_LAUNCH(adapter_low_kernel<T>, dim3((unsigned)blocks, (W + COLS - 1) / COLS, k_pieces(p.K)), 256, 0, s, p);
+    RFX_LAUNCH((adapter_up_kernel<T, TO>), dim3((unsigned)blocks, (p.N + OUT_COLS - 1) / OUT_COLS), 256, smem, s, p);
+    return 0;
+}
+
+}  // namespace
+
+// order [R], first [n + 2], tiles [max_tiles][3]; an id below -1 or from n on counts as none and sets *err.
+extern "C" int rfx_adapter_rows(const int* ids, int R, int n, int tile, int* order, int* first, int* tiles,
+                                int max_tiles, int* err, void* stream) {
+    if (R <= 0 || n <= 0 || tile <= 0 || max_tiles < min(R, n + 1) + R / tile) return RFX_ERR_BAD_ARG;
+    if (n > MAX_ADAPTERS) return RFX_ERR_UNSUPPORTED;
+    const size_t smem = ((size_t)(GROUP_THREADS / 32) * (n + 1) + 2 * (n + 2)) * sizeof(int);
+    cudaError_t e = cudaFuncSetAttribute(adapter_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    RFX_LAUNCH(adapter_rows_kernel, 1, GROUP_THREADS, smem, (cudaStream_t)stream, ids, R, n, tile, order, first, tiles,
+               max_tiles, err);
+    return 0;
+}
+
+// Floats of scratch that rfx_adapter_add needs.
+extern "C" long long rfx_adapter_low_floats(int R, int K, int parts, int rank) {
+    if (R <= 0 || K <= 0 || parts <= 0 || rank <= 0) return 0;
+    return (long long)k_pieces(K) * R * parts * rank;
+}
+
+// dt: of x, a and b; dt_out: of base and out (32-bit, or bfloat16 beside bfloat16).  ends[parts]: a part's last
+// column and one; woven: two parts, column by column.  low: rfx_adapter_low_floats(...) floats.
+extern "C" int rfx_adapter_add(const void* base, long long ld_base, void* out, long long ld_out, int dt_out, const void* x,
+                               long long ld_x, int dt, const void* a, int lda, const void* b, const float* scale,
+                               const int* ranks, const int* ends, int parts, int woven, const int* order,
+                               const int* tiles, int max_tiles, int tile, float* low, int R, int K, int N, int rank, int n,
+                               int* err, void* stream) {
+    if (R <= 0 || N <= 0) return 0;
+    if (K <= 0 || rank <= 0 || n <= 0 || tile <= 0 || max_tiles <= 0 || parts <= 0 || !low || lda < K || ld_x < K ||
+        ld_base < N || ld_out < N || (woven && (parts != 2 || N % 2)))
+        return RFX_ERR_BAD_ARG;
+    if (parts > MAX_PARTS || parts * rank > 1024 || (dt != RFX_DT_F32 && dt != RFX_DT_BF16) ||
+        (dt == RFX_DT_F32 && dt_out != RFX_DT_F32) || (dt_out != RFX_DT_F32 && dt_out != RFX_DT_BF16))
+        return RFX_ERR_UNSUPPORTED;
+    Args p{base, out, x, a, b, scale, ranks, order, tiles, low, ld_base, ld_out, ld_x, n, R, K, lda, N, rank, max_tiles,
+           tile, {}};
+    p.parts.n = parts;
+    p.parts.woven = woven;
+    for (int i = 0; i < parts; ++i) p.parts.end[i] = ends[i];
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dt == RFX_DT_F32) return fma_form<float, float>(p, s);
+    if (dt_out == RFX_DT_F32) return fma_form<__nv_bfloat16, float>(p, s);
+    return fma_form<__nv_bfloat16, __nv_bfloat16>(p, s);
+}

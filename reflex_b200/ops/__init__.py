@@ -203,7 +203,7 @@ def check_device_errors(device="cuda:0") -> None:
     if code:
         device_error_word(device).zero_()
         raise CudaError(f"a kernel reported an error (code {code}: a bounded wait that ran out, or a token "
-                        f"id outside the vocabulary); the step's results are not valid")
+                        f"id or an adapter outside its range); the step's results are not valid")
 
 
 def wait_probe(limit_ns: int, device="cuda:0") -> None:
@@ -398,6 +398,147 @@ def linear_geglu(x: torch.Tensor, weight_pairs: torch.Tensor) -> torch.Tensor:
         native.check(st, f"gemm_bf16_tc_geglu (R={R}, N={N}, K={K})")
         return y
     return swiglu(linear(x, weight_pairs), alternating=True, activation="gelu_tanh")
+
+
+# ------------------------------------------------------------------ adapters
+ADAPTER_STEP_ROWS = 256  # up to here rows go by tiles of 16, as requests that bring a token each; beyond by tiles of 128
+
+
+class AdapterRows:
+    """A step's rows by the adapter of their request (`adapter_rows`): `order` int32 [R], the rows of adapter 0,
+    then of 1, ..., then those without one, in order within each; `first` int32 [n + 2], where adapter a's begin
+    (`n` stands for none); `tiles` int32 [t, 3], these groups in tiles of at most `tile` rows: adapter, place in
+    `order`, rows; -1, 0, 0 behind the last."""
+
+    def __init__(self, order: torch.Tensor, first: torch.Tensor, tiles: torch.Tensor, tile: int):
+        self.order, self.first, self.tiles, self.tile = order, first, tiles, tile
+
+
+def adapter_rows(ids: torch.Tensor, n: int, tile: Optional[int] = None) -> AdapterRows:
+    """Groups rows by `ids` (int32 [R], 0 .. n - 1, -1: no adapter) for the products of `adapter_add`: once a
+    step, for all of them.  An id outside that range counts as none and is reported by `check_device_errors`."""
+    R = ids.numel()
+    if tile is None:
+        tile = 16 if R <= ADAPTER_STEP_ROWS else 128
+    if tile not in (16, 128):
+        raise InvalidInput(f"adapter_rows: tiles have 16 or 128 rows, not {tile}")
+    if ids.dim() != 1 or R == 0 or not 1 <= n <= 1024:
+        raise InvalidInput("adapter_rows: ids [rows], at least one, and 1 to 1024 adapters")
+    _on_current(ids, "ids")
+    t = min(R, n + 1) + R // tile
+    order = _new((R,), torch.int32, ids.device, keep=True)  # lives for the step
+    first = _new((n + 2,), torch.int32, ids.device, keep=True)
+    tiles = _new((t, 3), torch.int32, ids.device, keep=True)
+    st = native.lib().rfx_adapter_rows(_chk(ids, "ids", torch.int32), R, n, tile, order.data_ptr(), first.data_ptr(),
+                                       tiles.data_ptr(), t, device_error_word(ids.device).data_ptr(), _stream())
+    native.check(st, f"adapter_rows (R={R}, n={n})")
+    return AdapterRows(order, first, tiles, tile)
+
+
+class AdapterBank:
+    """The low-rank adapters of one projection, resident together.  `a` [n, parts, rank, K] and `b` [n, N, rank]
+    in the projection's type, `scale` float32 [n]: adapter i adds scale[i] b[i][c] . (a[i][part of c] x) to column
+    c of x's row.  `cols`: the columns of each part of a stacked projection (q | k | v), which sum to N, each part
+    with rows of `a` of its own; `woven`: two equal parts column by column (gate_0, up_0, gate_1, ...).  `ranks`
+    int32 [n]: adapters of a smaller rank, whose rows of `a` and columns of `b` beyond it are zero (and are not
+    read where that saves time).  Ranks and widths that the tensor-core kernels do not take as they are (no
+    multiple of 16, of 8) are padded with zeros here, once."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, cols, woven: bool = False,
+                 ranks: Optional[torch.Tensor] = None):
+        import ctypes
+
+        cols = tuple(int(c) for c in cols)
+        if a.dim() != 4 or b.dim() != 3:
+            raise InvalidInput("AdapterBank: a [n, parts, rank, K] and b [n, N, rank] are needed")
+        n, parts, rank, K = a.shape
+        N = sum(cols)
+        if parts != len(cols) or tuple(b.shape) != (n, N, rank) or min(cols, default=0) < 1:
+            raise InvalidInput(f"AdapterBank: a {tuple(a.shape)} and b {tuple(b.shape)} do not fit columns {cols}")
+        if a.dtype != b.dtype:
+            raise InvalidInput(f"AdapterBank: a is {a.dtype}, b is {b.dtype}")
+        dt_code(a.dtype)
+        if not (1 <= n <= 1024 and K >= 1 and 1 <= rank <= 256 and 1 <= parts <= 8) or parts * ((rank + 15) // 16 * 16) > 1024:
+            raise InvalidInput("AdapterBank: 1 to 1024 adapters, 1 to 8 parts, ranks of 1 to 256, parts * rank at most 1024")
+        if woven and (parts != 2 or cols[0] != cols[1]):
+            raise InvalidInput("AdapterBank: woven parts are two of as many columns")
+        if scale.numel() != n or (ranks is not None and ranks.numel() != n):
+            raise InvalidInput("AdapterBank: one scale, and one rank, per adapter")
+        self.n, self.rank, self.K, self.N, self.cols, self.woven = n, rank, K, N, cols, bool(woven)
+        self.dtype, self.device = a.dtype, a.device
+        if a.dtype == torch.bfloat16 and (rank % 16 or K % 8):
+            pad_r = -rank % 16
+            a = torch.nn.functional.pad(a, (0, -K % 8, 0, pad_r))
+            b = torch.nn.functional.pad(b, (0, pad_r))
+        _chk(a, "a")
+        _chk(b, "b")
+        _chk(scale, "scale", torch.float32)
+        _chk(ranks, "ranks", torch.int32)
+        for t, name in ((b, "b"), (scale, "scale"), (ranks, "ranks")):
+            if t is not None and t.device != a.device:
+                raise InvalidInput(f"AdapterBank: {name} lives on {t.device}, a on {a.device}")
+        self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
+        ends = [sum(cols[:i + 1]) for i in range(parts)]
+        self._ends = (ctypes.c_int * parts)(*ends)
+
+
+def _on_current(t: torch.Tensor, what: str) -> None:
+    """The launches go to the current device's current stream, so that is where the tensors have to live."""
+    if not t.is_cuda:
+        raise CudaError(f"{what} must live on the GPU (there is no CPU path)")
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise InvalidInput(f"{what} lives on {t.device}, but the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+def _rows_of(t: torch.Tensor, name: str) -> int:
+    """The elements from one row of a matrix to the next; a row's own lie side by side."""
+    _on_current(t, name)
+    if t.dim() != 2:
+        raise InvalidInput(f"{name} must be a matrix")
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise InvalidInput(f"{name}: a row's elements lie side by side, and rows do not overlap")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, rows: AdapterRows,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """base + scale_a B_a (A_a x), row by row with the row's own adapter a (`rows`); a row without one is base's.
+    `base` [R, N] float32, or bfloat16 beside a bfloat16 bank, is what the shared projection gave for `x` [R, K]
+    (the bank's type); the sum is taken in 32-bit and rounded once.  `out` may be `base` itself: rows without an
+    adapter are then left alone.  Rows of base, x and out may lie apart."""
+    R, K = x.shape
+    ld_x, ld_base = _rows_of(x, "x"), _rows_of(base, "base")
+    if K != bank.K or tuple(base.shape) != (R, bank.N):
+        raise InvalidInput(f"adapter_add: x [{R}, {bank.K}] and base [{R}, {bank.N}] are needed, "
+                           f"got {tuple(x.shape)} and {tuple(base.shape)}")
+    if x.dtype != bank.dtype:
+        raise InvalidInput(f"adapter_add: x is {x.dtype}, the adapters are {bank.dtype}")
+    if rows.order.numel() != R or rows.first.numel() != bank.n + 2:
+        raise InvalidInput(f"adapter_add: the rows were grouped for {rows.order.numel()} rows and "
+                           f"{rows.first.numel() - 2} adapters, not {R} and {bank.n}")
+    if not (x.device == base.device == bank.device == rows.order.device):
+        raise InvalidInput("adapter_add: x, base, the adapters and the rows live on one device")
+    if base.dtype != torch.float32 and base.dtype != bank.dtype:
+        raise InvalidInput(f"adapter_add: base is {base.dtype} beside adapters in {bank.dtype}")
+    if out is None:
+        out = _new((R, bank.N), base.dtype, base.device)
+        ld_out = bank.N
+    else:
+        ld_out = _rows_of(out, "out")
+        if out.shape != base.shape or out.dtype != base.dtype or out.device != base.device:
+            raise InvalidInput("adapter_add: out must be like base")
+    lib = native.lib()
+    rank = bank.a.shape[2]
+    parts = len(bank.cols)
+    low = _new((lib.rfx_adapter_low_floats(R, K, parts, rank),), torch.float32, x.device)
+    st = lib.rfx_adapter_add(
+        base.data_ptr(), ld_base, out.data_ptr(), ld_out, dt_code(base.dtype), x.data_ptr(), ld_x, dt_code(x.dtype),
+        bank.a.data_ptr(), bank.a.shape[3], bank.b.data_ptr(), bank.scale.data_ptr(),
+        0 if bank.ranks is None else bank.ranks.data_ptr(), bank._ends, parts, 1 if bank.woven else 0,
+        rows.order.data_ptr(), rows.tiles.data_ptr(), rows.tiles.shape[0], rows.tile, low.data_ptr(), R, K, bank.N, rank,
+        bank.n, device_error_word(x.device).data_ptr(), _stream())
+    native.check(st, f"adapter_add (R={R}, K={K}, N={bank.N}, rank={rank})")
+    return out
 
 
 # ----------------------------------------------------------------- attention
@@ -2326,4 +2467,34 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tenso
         _chk(uniform, "uniform", torch.float32), _chk(scratch, "scratch", torch.float32),
         _chk(work, "work", torch.uint8), out.data_ptr(), _stream())
     native.check(st, "sample")
+    return out
+
+
+def sample_rows(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tensor,
+                top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token a row, int32 [B], from float32 logits [B, V] (rows may lie apart), each row with its own rules:
+    `temperature` (<= 0 or NaN: the largest logit, ties to the highest index, as `argmax`), `top_k` int32 (<= 0:
+    off), `top_p` (>= 1: off), `min_p` (<= 0: off; tokens of at least min_p times the most probable one's
+    probability) and its random number `uniform` in [0, 1).  Top-p's mass is that of the whole vocabulary; among
+    equal logits the lower index is kept first; the draw walks the kept tokens in index order.  Logits of -inf or
+    NaN are never picked; a row with nothing else gives 0.  One launch, without working memory; exponentials and
+    sums are 64-bit, so a token is the one that exact arithmetic picks but for draws within 1e-12 of a border."""
+    ld = _rows_of(logits, "logits")
+    B, V = logits.shape
+    if logits.dtype != torch.float32:
+        raise InvalidInput(f"logits must be torch.float32, got {logits.dtype}")
+    if B == 0 or V == 0:
+        raise InvalidInput("sample_rows: no rows, or no vocabulary")
+    if out is None:
+        out = torch.empty((B,), dtype=torch.int32, device=logits.device)
+    ptrs = []
+    for t, name, dtype in ((temperature, "temperature", torch.float32), (uniform, "uniform", torch.float32),
+                           (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                           (min_p, "min_p", torch.float32), (out, "out", torch.int32)):
+        ptrs.append(_chk(t, name, dtype))
+        if t is not None and (t.numel() != B or t.device != logits.device):
+            raise InvalidInput(f"sample_rows: {name} must have a number for each of the {B} rows, beside the logits")
+    st = native.lib().rfx_sample_rows(logits.data_ptr(), ld, B, V, *ptrs, _stream())
+    native.check(st, f"sample_rows (B={B}, V={V})")
     return out

@@ -50,7 +50,7 @@ class PendingIds:
 
                 self.err_dev.zero_()
                 raise CudaError(f"a kernel reported an error (code {code}: a bounded wait that ran out, or a "
-                                f"token id outside the vocabulary); the step's results are not valid")
+                                f"token id or an adapter outside its range); the step's results are not valid")
         return self.host.tolist()
 
 
