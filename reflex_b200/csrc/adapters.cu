@@ -235,8 +235,8 @@ int fma_form(const Args& p, cudaStream_t s) {
     if (blocks > 0x7fffffffLL || (p.N + OUT_COLS - 1) / OUT_COLS > 65535 || (W + COLS - 1) / COLS > 65535)
         return RFX_ERR_UNSUPPORTED;
     const size_t smem = (size_t)ROWS * W * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(adapter_up_kernel<T, TO>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
+    static SmemLimit limit;
+    cudaError_t e = limit.raise(adapter_up_kernel<T, TO>, smem);
     if (e != cudaSuccess) return (int)e;
     RFX_LAUNCH(adapter_low_kernel<T>, dim3((unsigned)blocks, (W + COLS - 1) / COLS, k_pieces(p.K)), 256, 0, s, p);
     RFX_LAUNCH((adapter_up_kernel<T, TO>), dim3((unsigned)blocks, (p.N + OUT_COLS - 1) / OUT_COLS), 256, smem, s, p);
@@ -251,40 +251,51 @@ extern "C" int rfx_adapter_rows(const int* ids, int R, int n, int tile, int* ord
     if (R <= 0 || n <= 0 || tile <= 0 || max_tiles < min(R, n + 1) + R / tile) return RFX_ERR_BAD_ARG;
     if (n > MAX_ADAPTERS) return RFX_ERR_UNSUPPORTED;
     const size_t smem = ((size_t)(GROUP_THREADS / 32) * (n + 1) + 2 * (n + 2)) * sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(adapter_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemLimit limit;
+    cudaError_t e = limit.raise(adapter_rows_kernel, smem);
     if (e != cudaSuccess) return (int)e;
     RFX_LAUNCH(adapter_rows_kernel, 1, GROUP_THREADS, smem, (cudaStream_t)stream, ids, R, n, tile, order, first, tiles,
                max_tiles, err);
     return 0;
 }
 
-// Floats of scratch that rfx_adapter_add needs.
-extern "C" long long rfx_adapter_low_floats(int R, int K, int parts, int rank) {
-    if (R <= 0 || K <= 0 || parts <= 0 || rank <= 0) return 0;
-    return (long long)k_pieces(K) * R * parts * rank;
+// A projection's adapters (the fields of ops.AdapterBank's `_Bank`).
+struct AdapterBank {
+    const void *a, *b;
+    const float* scale;
+    const int* ranks;
+    int n, K, lda, N, rank, parts, woven, dt;
+    int ends[MAX_PARTS];  // a part's last column and one
+};
+
+// Floats of scratch that rfx_adapter_add needs in a form: 0 the products in 32-bit multiply-adds, 1 tiles of
+// 16 rows on the tensor cores.
+extern "C" long long rfx_adapter_low_floats(const AdapterBank* k, int R, int form) {
+    if (R <= 0 || !k || k->K <= 0 || form != 0) return 0;
+    return (long long)k_pieces(k->K) * R * k->parts * k->rank;
 }
 
-// dt: of x, a and b; dt_out: of base and out (32-bit, or bfloat16 beside bfloat16).  ends[parts]: a part's last
-// column and one; woven: two parts, column by column.  low: rfx_adapter_low_floats(...) floats.
-extern "C" int rfx_adapter_add(const void* base, long long ld_base, void* out, long long ld_out, int dt_out, const void* x,
-                               long long ld_x, int dt, const void* a, int lda, const void* b, const float* scale,
-                               const int* ranks, const int* ends, int parts, int woven, const int* order,
-                               const int* tiles, int max_tiles, int tile, float* low, int R, int K, int N, int rank, int n,
-                               int* err, void* stream) {
-    if (R <= 0 || N <= 0) return 0;
-    if (K <= 0 || rank <= 0 || n <= 0 || tile <= 0 || max_tiles <= 0 || parts <= 0 || !low || lda < K || ld_x < K ||
-        ld_base < N || ld_out < N || (woven && (parts != 2 || N % 2)))
+// dt_out: of base and out (32-bit, or bfloat16 beside bfloat16).
+extern "C" int rfx_adapter_add(const AdapterBank* k, const int* order, const int* tiles, int max_tiles, int tile,
+                               const void* base, long long ld_base, void* out, long long ld_out, int dt_out, const void* x,
+                               long long ld_x, float* low, int R, int form, int* err, void* stream) {
+    if (!k) return RFX_ERR_BAD_ARG;
+    if (R <= 0 || k->N <= 0) return 0;
+    if (k->K <= 0 || k->rank <= 0 || k->n <= 0 || tile <= 0 || max_tiles <= 0 || k->parts <= 0 || k->lda < k->K ||
+        ld_x < k->K || ld_base < k->N || ld_out < k->N || (k->woven && (k->parts != 2 || k->N % 2)))
         return RFX_ERR_BAD_ARG;
-    if (parts > MAX_PARTS || parts * rank > 1024 || (dt != RFX_DT_F32 && dt != RFX_DT_BF16) ||
-        (dt == RFX_DT_F32 && dt_out != RFX_DT_F32) || (dt_out != RFX_DT_F32 && dt_out != RFX_DT_BF16))
+    if (k->parts > MAX_PARTS || k->parts * k->rank > 1024 || (k->dt != RFX_DT_F32 && k->dt != RFX_DT_BF16) ||
+        (k->dt == RFX_DT_F32 && dt_out != RFX_DT_F32) || (dt_out != RFX_DT_F32 && dt_out != RFX_DT_BF16))
         return RFX_ERR_UNSUPPORTED;
-    Args p{base, out, x, a, b, scale, ranks, order, tiles, low, ld_base, ld_out, ld_x, n, R, K, lda, N, rank, max_tiles,
-           tile, {}};
-    p.parts.n = parts;
-    p.parts.woven = woven;
-    for (int i = 0; i < parts; ++i) p.parts.end[i] = ends[i];
+    Args p{base, out, x, k->a, k->b, k->scale, k->ranks, order, tiles, low, ld_base, ld_out, ld_x, k->n, R, k->K, k->lda,
+           k->N, k->rank, max_tiles, tile, {}};
+    p.parts.n = k->parts;
+    p.parts.woven = k->woven;
+    for (int i = 0; i < k->parts; ++i) p.parts.end[i] = k->ends[i];
     cudaStream_t s = (cudaStream_t)stream;
-    if (dt == RFX_DT_F32) return fma_form<float, float>(p, s);
+    if (form == 1) return k->dt == RFX_DT_BF16 && step_takes(p) ? step_form(p, dt_out, s) : RFX_ERR_UNSUPPORTED;
+    if (form != 0 || !low) return RFX_ERR_BAD_ARG;
+    if (k->dt == RFX_DT_F32) return fma_form<float, float>(p, s);
     if (dt_out == RFX_DT_F32) return fma_form<__nv_bfloat16, float>(p, s);
     return fma_form<__nv_bfloat16, __nv_bfloat16>(p, s);
 }

@@ -51,4 +51,8 @@ struct Args {
     }
 };
 
+// tiles of 16 rows, bfloat16 (adapters_step.cu)
+bool step_takes(const Args& p);
+int step_form(const Args& p, int dt_out, cudaStream_t s);
+
 }  // namespace adapters

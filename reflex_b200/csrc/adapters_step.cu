@@ -1,0 +1,281 @@
+// The adapters of a step's requests, a row or a few each: tiles of at most 16 rows, bfloat16, one launch.
+//
+// A thread-block cluster takes a tile and both products.  Each of its eight CTAs multiplies the tile's rows
+// with A over an eighth of K on the tensor cores (m16n8k16: 16 rows, 8 rank rows), its warps over every eighth
+// 32 of that; the partial sums meet in shared memory and, over the cluster, in distributed shared memory, in
+// rank order; then each CTA multiplies the low-rank rows with its share of B's columns and adds the base.
+// Nothing but the result goes back to memory, and there is one launch where two would have to follow one another.
+//
+// It is latency and the adapters' bytes that count (an adapter of rank 16 beside 4,096 x 6,144: 0.6 MB): operands
+// come from memory straight into fragments by 16- and 8-byte loads, with k permuted alike on both sides so
+// that a lane's elements lie side by side, and a warp's first columns of B and of the base are on their way
+// before the cluster meets.
+//
+// The low-rank rows are kept in 32 bits and go into the second product as three bfloat16 parts (24 bits).
+// How K is cut depends on K alone, and a row's sums on nothing else in the tile, so a row has the same bits
+// whatever shares its step.
+#include <cooperative_groups.h>
+
+#include "adapters.cuh"
+#include "attn_mma.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+using namespace rfx;
+using namespace adapters;
+
+constexpr int CLUSTER = 8, THREADS = 256, WARPS = THREADS / 32, TILE = 16;
+constexpr int CHUNK = 8;                    // tiles of 8 rank rows that a warp sums at a time
+constexpr int RED_LD = CHUNK * 8 + 4;
+constexpr int GROUP = 32;                   // columns a warp makes at a time
+constexpr int AHEAD = 4;                    // steps of 16 along the rank whose B is loaded before the cluster meets
+
+__host__ __device__ inline int k_slice(int K) { return ((K + CLUSTER - 1) / CLUSTER + 31) / 32 * 32; }
+// floats of the partial rows, and the three parts' bfloat16s
+inline size_t step_smem(int W) {
+    return (size_t)WARPS * TILE * RED_LD * 4 + (size_t)TILE * W * 4 + (size_t)3 * TILE * (W + 8) * 2;
+}
+
+__device__ __forceinline__ uint4 load16(const __nv_bfloat16* p, bool valid) {
+    return valid ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
+}
+
+template <typename TO>
+__device__ __forceinline__ void load8(const TO* p, float (&v)[8]) {
+    const float4 a = load4(p), b = load4(p + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+template <typename TO>
+__global__ void __launch_bounds__(THREADS) adapter_step_kernel(const Args p, int groups, int vec) {
+    extern __shared__ __align__(16) uint8_t dynamic[];
+    __shared__ int rows[TILE];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int W = p.parts.n * p.rank, LDV = W + 8;
+    float* red = reinterpret_cast<float*>(dynamic);                                       // [WARPS][TILE][RED_LD]
+    float* part_v = red + WARPS * TILE * RED_LD;                                          // [TILE][W]
+    __nv_bfloat16* vs = reinterpret_cast<__nv_bfloat16*>(part_v + TILE * W);              // [3][TILE][LDV]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    pdl_prologue();
+    const Tile tile = load_tile(p.tiles, blockIdx.y);
+    if (tile.adapter < 0) return;  // (the same for the whole cluster)
+    const bool none = tile.adapter >= p.n;
+    if (none && p.out == p.base) return;
+    const int count = min(tile.count, TILE), c = cluster.block_rank();
+    if (tid < TILE) rows[tid] = p.order[tile.place + min(tid, count - 1)];
+    const int rank = none ? 0 : p.rank_of(tile.adapter);
+    const int per = (rank + 7) / 8, steps = (rank + 15) / 16, tiles = per * p.parts.n;
+    __syncthreads();
+
+    // a warp's columns: groups of 32 from the start of a part (woven: of the whole), lane (g, t) has columns
+    // 8 t .. 8 t + 7 of rows g and g + 8
+    const __nv_bfloat16* b = (const __nv_bfloat16*)p.b + (size_t)tile.adapter * p.N * p.rank;
+    int group = (blockIdx.x * CLUSTER + c) * WARPS + warp;
+    const int stride = gridDim.x * CLUSTER * WARPS;
+    auto locate = [&](int q, int& col, int& end, int& part) {
+        int first = 0;
+        part = 0;
+        if (!p.parts.woven)
+            while (true) {
+                const int n = (p.parts.end[part] - first + GROUP - 1) / GROUP;
+                if (q < n || part + 1 == p.parts.n) break;
+                q -= n;
+                first = p.parts.end[part++];
+            }
+        col = first + q * GROUP;
+        end = p.parts.woven ? p.N : p.parts.end[part];
+    };
+    auto load_b = [&](int col, int end, int s, int j) {  // step s of tile j: columns col + 4 n + j
+        const int at = min(col + 4 * g + j, end - 1);
+        return __ldg(reinterpret_cast<const uint2*>(b + (size_t)at * p.rank + s * 16 + t * 4));
+    };
+    const TO* base = (const TO*)p.base;
+    TO* out = (TO*)p.out;
+    auto load_base = [&](int col, int end, int r, float (&v)[8]) {
+        const int at = col + 8 * t;
+        if (r < count) {
+            const TO* src = base + (size_t)rows[r] * p.ld_base + at;
+            if (vec && at + 8 <= end && (at & 7) == 0) load8(src, v);
+            else
+                for (int i = 0; i < 8; ++i) v[i] = at + i < end ? ld(src, i) : 0.f;
+        }
+    };
+    uint2 ahead[AHEAD][4];
+    float base_lo[8], base_hi[8];
+    int col = 0, end = 0, part = 0;
+    const bool any = group < groups;
+    if (any) {
+        locate(group, col, end, part);
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s)
+            if (s < steps)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ahead[s][j] = load_b(col, end, s, j);
+        load_base(col, end, g, base_lo);
+        load_base(col, end, g + 8, base_hi);
+    }
+
+    if (!none) {
+        // ---- the low-rank rows over this CTA's slice of K
+        const __nv_bfloat16* a = (const __nv_bfloat16*)p.a + (size_t)tile.adapter * W * p.lda;
+        const __nv_bfloat16* x = (const __nv_bfloat16*)p.x;
+        const __nv_bfloat16 *x0 = x + (size_t)rows[g] * p.ld_x, *x1 = x + (size_t)rows[g + 8] * p.ld_x;
+        const int k0 = c * k_slice(p.K), k1 = min(p.K, k0 + k_slice(p.K));
+        for (int i = tid; i < 3 * TILE * LDV / 2; i += THREADS) reinterpret_cast<uint32_t*>(vs)[i] = 0u;
+        for (int n0 = 0; n0 < tiles; n0 += CHUNK) {
+            const int here = min(CHUNK, tiles - n0);
+            float acc[CHUNK][4] = {};
+            const __nv_bfloat16* a_row[CHUNK];
+#pragma unroll
+            for (int i = 0; i < CHUNK; ++i) {
+                const int n = n0 + min(i, here - 1), s = n / per;
+                a_row[i] = a + (size_t)(s * p.rank + (n - s * per) * 8 + g) * p.lda;
+            }
+#pragma unroll 2
+            for (int k = k0 + warp * 32; k < k1; k += WARPS * 32) {
+                const int kt = k + t * 8;
+                const bool in = kt < k1;
+                const uint4 xa = load16(x0 + kt, in && g < count), xb = load16(x1 + kt, in && g + 8 < count);
+                uint4 w[CHUNK];
+#pragma unroll
+                for (int i = 0; i < CHUNK; ++i) w[i] = load16(a_row[i] + kt, in && i < here);
+                const uint32_t f0[4] = {xa.x, xb.x, xa.y, xb.y}, f1[4] = {xa.z, xb.z, xa.w, xb.w};
+#pragma unroll
+                for (int i = 0; i < CHUNK; ++i) {
+                    attn::mma_bf16(acc[i], f0, w[i].x, w[i].y);
+                    attn::mma_bf16(acc[i], f1, w[i].z, w[i].w);
+                }
+            }
+            __syncthreads();  // the sums of the chunk before have been read
+            float* mine = red + warp * TILE * RED_LD;
+#pragma unroll
+            for (int i = 0; i < CHUNK; ++i) {
+                store2(mine + g * RED_LD + i * 8 + t * 2, acc[i][0], acc[i][1]);
+                store2(mine + (g + 8) * RED_LD + i * 8 + t * 2, acc[i][2], acc[i][3]);
+            }
+            __syncthreads();
+            for (int i = tid; i < count * CHUNK * 8; i += THREADS) {
+                const int r = i / (CHUNK * 8), n = i % (CHUNK * 8);
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) v += red[(w * TILE + r) * RED_LD + n];
+                if (n < here * 8) part_v[r * W + n0 * 8 + n] = v;
+            }
+        }
+        cluster.sync();
+        // ---- the cluster's sums, in three parts of bfloat16
+        for (int i = tid; i < count * tiles * 8; i += THREADS) {
+            const int r = i / (tiles * 8), n = i - r * tiles * 8;
+            float v = 0.f;
+#pragma unroll
+            for (int q = 0; q < CLUSTER; ++q) v += cluster.map_shared_rank(part_v, q)[r * W + n];
+            const int s = n / (per * 8), at = r * LDV + s * p.rank + n - s * per * 8;
+            const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+            const float rest = v - __bfloat162float(hi);
+            const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
+            vs[at] = hi;
+            vs[TILE * LDV + at] = mid;
+            vs[2 * TILE * LDV + at] = __float2bfloat16_rn(rest - __bfloat162float(mid));
+        }
+        cluster.sync();  // no CTA leaves while another reads its sums
+    }
+
+    // ---- the columns
+    const float scale = none ? 0.f : p.scale[tile.adapter];
+    for (bool first = true; group < groups; group += stride, first = false) {
+        if (!first) {
+            locate(group, col, end, part);
+            load_base(col, end, g, base_lo);
+            load_base(col, end, g + 8, base_hi);
+        }
+        float acc[4][4] = {};
+        for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+            if (!first || s0)
+#pragma unroll
+                for (int s = 0; s < AHEAD; ++s)
+                    if (s0 + s < steps)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) ahead[s][j] = load_b(col, end, s0 + s, j);
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s)
+                if (s0 + s < steps)
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) {
+                        const __nv_bfloat16* v = vs + q * TILE * LDV + (s0 + s) * 16 + t * 4;
+                        auto frag = [&](int sp, uint32_t (&f)[4]) {
+                            const uint2 lo = *reinterpret_cast<const uint2*>(v + g * LDV + sp * p.rank);
+                            const uint2 hi = *reinterpret_cast<const uint2*>(v + (g + 8) * LDV + sp * p.rank);
+                            f[0] = lo.x, f[1] = hi.x, f[2] = lo.y, f[3] = hi.y;
+                        };
+                        uint32_t f[4], odd[4];
+                        frag(part, f);
+                        if (p.parts.woven) frag(1, odd);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if ((j & 1) && p.parts.woven) attn::mma_bf16(acc[j], odd, ahead[s][j].x, ahead[s][j].y);
+                            else attn::mma_bf16(acc[j], f, ahead[s][j].x, ahead[s][j].y);
+                        }
+                    }
+        }
+        auto store = [&](int r, const float (&y)[8], int h) {
+            const int at = col + 8 * t;
+            if (r >= count) return;
+            TO* dst = out + (size_t)rows[r] * p.ld_out + at;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = none ? y[i] : fmaf(scale, acc[i & 3][h + (i >> 2)], y[i]);
+            if (vec && at + 8 <= end && (at & 7) == 0) {
+                store4(dst, make_float4(v[0], v[1], v[2], v[3]));
+                store4(dst + 4, make_float4(v[4], v[5], v[6], v[7]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (at + i < end) st(dst, i, v[i]);
+            }
+        };
+        store(g, base_lo, 0);
+        store(g + 8, base_hi, 2);
+    }
+}
+
+template <typename TO>
+int go(const Args& p, cudaStream_t s) {
+    const int W = p.parts.n * p.rank;
+    int groups = 0;
+    for (int i = 0, first = 0; i < p.parts.n; first = p.parts.end[i++])
+        groups += (p.parts.end[i] - first + GROUP - 1) / GROUP;
+    if (p.parts.woven) groups = (p.N + GROUP - 1) / GROUP;
+    // Several clusters share a tile's columns (each makes the low-rank rows for itself, A comes from L2) until
+    // the grid holds a CTA for every SM, or every warp has one group of columns.
+    int share = (sm_count() + CLUSTER * p.max_tiles - 1) / (CLUSTER * p.max_tiles);
+    const int most = (groups + CLUSTER * WARPS - 1) / (CLUSTER * WARPS);
+    if (share > most) share = most;
+    const size_t smem = step_smem(W);
+    // rows of base and out by 16 bytes
+    const size_t align = (size_t)p.base | (size_t)p.out | (size_t)(p.ld_base * sizeof(TO)) | (size_t)(p.ld_out * sizeof(TO));
+    const int vec = (align & 15) == 0;
+    static SmemLimit limit;
+    cudaError_t e = limit.raise(adapter_step_kernel<TO>, smem);
+    if (e == cudaSuccess)
+        e = launch(adapter_step_kernel<TO>, dim3(share, p.max_tiles, CLUSTER), THREADS, smem, s, CLUSTER, p, groups, vec);
+    return (int)e;
+}
+
+}  // namespace
+
+namespace adapters {
+
+// Whether the cluster form takes these: x, a and b by 16 bytes, ranks in sixteens.
+bool step_takes(const Args& p) {
+    const size_t align = (size_t)p.x | (size_t)p.a | (size_t)p.b | (size_t)(p.ld_x * 2) | (size_t)(p.lda * 2);
+    return p.tile == TILE && (align & 15) == 0 && p.K % 8 == 0 && p.rank % 16 == 0 && p.max_tiles <= 65535 &&
+           step_smem(p.parts.n * p.rank) <= 220 * 1024;
+}
+
+int step_form(const Args& p, int dt_out, cudaStream_t s) {
+    return dt_out == RFX_DT_F32 ? go<float>(p, s) : go<__nv_bfloat16>(p, s);
+}
+
+}  // namespace adapters

@@ -68,6 +68,23 @@ inline int sm_count() {
     return n;
 }
 
+// The dynamic shared memory that one kernel may ask for, raised when a launch asks for more than any before
+// it: one static object a kernel, so that a call does not pay for the attribute again.
+struct SmemLimit {
+    int have[16] = {};
+    template <typename K>
+    cudaError_t raise(K kernel, size_t bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        int* h = dev >= 0 && dev < 16 ? &have[dev] : nullptr;
+        if (h && *h >= (int)bytes) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess && h) *h = (int)bytes;
+        return e;
+    }
+};
+
 // Launch with the library's attributes; cluster_z > 1 asks for a thread-block
 // cluster of (1, 1, cluster_z).
 template <typename... KArgs, typename... Args>

@@ -412,7 +412,8 @@ extern "C" int rfx_sample_rows(const float* logits, long long ld, int B, int V, 
     Params p{logits, ld, V, chunk, temperature, uniform, top_p, min_p, top_k, out};
     auto kernel = staged ? sample_rows_kernel<true> : sample_rows_kernel<false>;
     const size_t smem = hist + (staged ? piece : 0);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemLimit limits[2];
+    cudaError_t e = limits[staged].raise(kernel, smem);
     if (e == cudaSuccess)
         e = launch(kernel, dim3(B, 1, C), THREADS, smem, (cudaStream_t)stream, C, p);
     return (int)e;

@@ -412,6 +412,8 @@ class AdapterRows:
 
     def __init__(self, order: torch.Tensor, first: torch.Tensor, tiles: torch.Tensor, tile: int):
         self.order, self.first, self.tiles, self.tile = order, first, tiles, tile
+        self.n_rows, self.n, self.n_tiles = order.numel(), first.numel() - 2, tiles.shape[0]
+        self.order_ptr, self.tiles_ptr = order.data_ptr(), tiles.data_ptr()
 
 
 def adapter_rows(ids: torch.Tensor, n: int, tile: Optional[int] = None) -> AdapterRows:
@@ -478,8 +480,18 @@ class AdapterBank:
             if t is not None and t.device != a.device:
                 raise InvalidInput(f"AdapterBank: {name} lives on {t.device}, a on {a.device}")
         self.a, self.b, self.scale, self.ranks = a, b, scale, ranks
-        ends = [sum(cols[:i + 1]) for i in range(parts)]
-        self._ends = (ctypes.c_int * parts)(*ends)
+        rank, lda = a.shape[2], a.shape[3]
+        # what the kernels have to know of it, in one piece (csrc/adapters.cu)
+        self._desc = (ctypes.c_longlong * 12)(a.data_ptr(), b.data_ptr(), scale.data_ptr(),
+                                              0 if ranks is None else ranks.data_ptr())
+        ints = (ctypes.c_int * 16).from_buffer(self._desc, 32)
+        ints[:8 + parts] = [n, K, lda, N, rank, parts, int(self.woven), dt_code(a.dtype)] + [
+            sum(cols[:i + 1]) for i in range(parts)]
+        self._ptr = ctypes.addressof(self._desc)
+        self._pieces = rank * parts
+        self._tensor_cores = (a.dtype == torch.bfloat16 and K % 8 == 0 and (a.data_ptr() | b.data_ptr()) % 16 == 0)
+        self._err = device_error_word(a.device).data_ptr()
+        self._index = a.get_device()
 
 
 def _on_current(t: torch.Tensor, what: str) -> None:
@@ -492,6 +504,8 @@ def _on_current(t: torch.Tensor, what: str) -> None:
 
 def _rows_of(t: torch.Tensor, name: str) -> int:
     """The elements from one row of a matrix to the next; a row's own lie side by side."""
+    if t.dim() == 2 and t.is_contiguous() and t.get_device() == torch._C._cuda_getDevice():
+        return t.shape[1]
     _on_current(t, name)
     if t.dim() != 2:
         raise InvalidInput(f"{name} must be a matrix")
@@ -506,38 +520,41 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, rows: Ad
     `base` [R, N] float32, or bfloat16 beside a bfloat16 bank, is what the shared projection gave for `x` [R, K]
     (the bank's type); the sum is taken in 32-bit and rounded once.  `out` may be `base` itself: rows without an
     adapter are then left alone.  Rows of base, x and out may lie apart."""
-    R, K = x.shape
     ld_x, ld_base = _rows_of(x, "x"), _rows_of(base, "base")
-    if K != bank.K or tuple(base.shape) != (R, bank.N):
+    R, K = x.shape
+    if K != bank.K or base.shape[0] != R or base.shape[1] != bank.N:
         raise InvalidInput(f"adapter_add: x [{R}, {bank.K}] and base [{R}, {bank.N}] are needed, "
                            f"got {tuple(x.shape)} and {tuple(base.shape)}")
     if x.dtype != bank.dtype:
         raise InvalidInput(f"adapter_add: x is {x.dtype}, the adapters are {bank.dtype}")
-    if rows.order.numel() != R or rows.first.numel() != bank.n + 2:
-        raise InvalidInput(f"adapter_add: the rows were grouped for {rows.order.numel()} rows and "
-                           f"{rows.first.numel() - 2} adapters, not {R} and {bank.n}")
-    if not (x.device == base.device == bank.device == rows.order.device):
+    if rows.n_rows != R or rows.n != bank.n:
+        raise InvalidInput(f"adapter_add: the rows were grouped for {rows.n_rows} rows and {rows.n} adapters, "
+                           f"not {R} and {bank.n}")
+    if bank._index != x.get_device() or rows.order.get_device() != bank._index:
         raise InvalidInput("adapter_add: x, base, the adapters and the rows live on one device")
-    if base.dtype != torch.float32 and base.dtype != bank.dtype:
-        raise InvalidInput(f"adapter_add: base is {base.dtype} beside adapters in {bank.dtype}")
+    dtype = base.dtype
+    if dtype != torch.float32 and dtype != bank.dtype:
+        raise InvalidInput(f"adapter_add: base is {dtype} beside adapters in {bank.dtype}")
     if out is None:
-        out = _new((R, bank.N), base.dtype, base.device)
+        out = _new((R, bank.N), dtype, base.device)
         ld_out = bank.N
     else:
         ld_out = _rows_of(out, "out")
-        if out.shape != base.shape or out.dtype != base.dtype or out.device != base.device:
+        if out.shape != base.shape or out.dtype != dtype:
             raise InvalidInput("adapter_add: out must be like base")
+    xp = x.data_ptr()
+    form = 1 if rows.tile == 16 and bank._tensor_cores and (xp | ld_x * 2) % 16 == 0 else 0
     lib = native.lib()
-    rank = bank.a.shape[2]
-    parts = len(bank.cols)
-    low = _new((lib.rfx_adapter_low_floats(R, K, parts, rank),), torch.float32, x.device)
+    low = 0
+    if form == 0:
+        scratch = _new((lib.rfx_adapter_low_floats(bank._ptr, R, form),), torch.float32, x.device)
+        low = scratch.data_ptr()
     st = lib.rfx_adapter_add(
-        base.data_ptr(), ld_base, out.data_ptr(), ld_out, dt_code(base.dtype), x.data_ptr(), ld_x, dt_code(x.dtype),
-        bank.a.data_ptr(), bank.a.shape[3], bank.b.data_ptr(), bank.scale.data_ptr(),
-        0 if bank.ranks is None else bank.ranks.data_ptr(), bank._ends, parts, 1 if bank.woven else 0,
-        rows.order.data_ptr(), rows.tiles.data_ptr(), rows.tiles.shape[0], rows.tile, low.data_ptr(), R, K, bank.N, rank,
-        bank.n, device_error_word(x.device).data_ptr(), _stream())
-    native.check(st, f"adapter_add (R={R}, K={K}, N={bank.N}, rank={rank})")
+        bank._ptr, rows.order_ptr, rows.tiles_ptr, rows.n_tiles, rows.tile, base.data_ptr(), ld_base, out.data_ptr(),
+        ld_out, F32 if dtype is torch.float32 else BF16, xp, ld_x, low, R, form, bank._err, _stream())
+    if st:
+        native.check(st, f"adapter_add (R={R}, K={K}, N={bank.N}, rank={bank.rank})")
+    native.LAUNCHES += 1
     return out
 
 
@@ -2488,13 +2505,17 @@ def sample_rows(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.
         raise InvalidInput("sample_rows: no rows, or no vocabulary")
     if out is None:
         out = torch.empty((B,), dtype=torch.int32, device=logits.device)
-    ptrs = []
-    for t, name, dtype in ((temperature, "temperature", torch.float32), (uniform, "uniform", torch.float32),
-                           (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
-                           (min_p, "min_p", torch.float32), (out, "out", torch.int32)):
-        ptrs.append(_chk(t, name, dtype))
-        if t is not None and (t.numel() != B or t.device != logits.device):
+    at = logits.get_device()
+
+    def ptr(t, name, dtype):
+        p = _chk(t, name, dtype)
+        if p and (t.numel() != B or t.get_device() != at):
             raise InvalidInput(f"sample_rows: {name} must have a number for each of the {B} rows, beside the logits")
-    st = native.lib().rfx_sample_rows(logits.data_ptr(), ld, B, V, *ptrs, _stream())
-    native.check(st, f"sample_rows (B={B}, V={V})")
+        return p
+
+    st = native.lib().rfx_sample_rows(
+        logits.data_ptr(), ld, B, V, ptr(temperature, "temperature", torch.float32),
+        ptr(uniform, "uniform", torch.float32), ptr(top_k, "top_k", torch.int32), ptr(top_p, "top_p", torch.float32),
+        ptr(min_p, "min_p", torch.float32), ptr(out, "out", torch.int32), _stream())
+    native.check(st, "sample_rows")
     return out

@@ -217,9 +217,8 @@ _SIGNATURES = {
     "rfx_sample_rows": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                         c_void_p],
     "rfx_adapter_rows": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
-    "rfx_adapter_add": [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int, c_void_p, c_int,
-                        c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p,
-                        c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+    "rfx_adapter_add": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int,
+                        c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_void_p],
     "rfx_sample": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                    c_void_p, c_void_p, c_void_p, c_void_p],
 }
@@ -262,7 +261,7 @@ def lib() -> ctypes.CDLL:
         handle.rfx_delta_rule_chunk_floats.restype = c_longlong
         handle.rfx_sm_count.argtypes = []
         handle.rfx_sm_count.restype = c_int
-        handle.rfx_adapter_low_floats.argtypes = [c_int] * 4
+        handle.rfx_adapter_low_floats.argtypes = [c_void_p, c_int, c_int]
         handle.rfx_adapter_low_floats.restype = c_longlong
         handle.rfx_sample_work_bytes.argtypes = [c_int, c_int]
         handle.rfx_sample_work_bytes.restype = c_longlong
