@@ -269,9 +269,10 @@ struct AdapterBank {
 };
 
 // Floats of scratch that rfx_adapter_add needs in a form: 0 the products in 32-bit multiply-adds, 1 tiles of
-// 16 rows on the tensor cores.
-extern "C" long long rfx_adapter_low_floats(const AdapterBank* k, int R, int form) {
-    if (R <= 0 || !k || k->K <= 0 || form != 0) return 0;
+// 16 rows and 2 tiles of 128 rows on the tensor cores.
+extern "C" long long rfx_adapter_low_floats(const AdapterBank* k, int R, int max_tiles, int form) {
+    if (R <= 0 || max_tiles <= 0 || !k || k->K <= 0 || form == 1) return 0;
+    if (form == 2) return prompt_low_floats(R, k->K, k->parts * k->rank, max_tiles);
     return (long long)k_pieces(k->K) * R * k->parts * k->rank;
 }
 
@@ -294,6 +295,8 @@ extern "C" int rfx_adapter_add(const AdapterBank* k, const int* order, const int
     for (int i = 0; i < k->parts; ++i) p.parts.end[i] = k->ends[i];
     cudaStream_t s = (cudaStream_t)stream;
     if (form == 1) return k->dt == RFX_DT_BF16 && step_takes(p) ? step_form(p, dt_out, s) : RFX_ERR_UNSUPPORTED;
+    if (form == 2 && low)
+        return k->dt == RFX_DT_BF16 && prompt_takes(p) ? prompt_form(p, dt_out, err, s) : RFX_ERR_UNSUPPORTED;
     if (form != 0 || !low) return RFX_ERR_BAD_ARG;
     if (k->dt == RFX_DT_F32) return fma_form<float, float>(p, s);
     if (dt_out == RFX_DT_F32) return fma_form<__nv_bfloat16, float>(p, s);

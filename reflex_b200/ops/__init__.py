@@ -488,8 +488,10 @@ class AdapterBank:
         ints[:8 + parts] = [n, K, lda, N, rank, parts, int(self.woven), dt_code(a.dtype)] + [
             sum(cols[:i + 1]) for i in range(parts)]
         self._ptr = ctypes.addressof(self._desc)
-        self._pieces = rank * parts
-        self._tensor_cores = (a.dtype == torch.bfloat16 and K % 8 == 0 and (a.data_ptr() | b.data_ptr()) % 16 == 0)
+        # which tiles the tensor cores take (bfloat16 rows on 16 bytes): of 16 rows, of 128 rows
+        tc = a.dtype == torch.bfloat16 and K % 8 == 0 and (a.data_ptr() | b.data_ptr()) % 16 == 0
+        self._form = {16: 1 if tc else 0,
+                      128: 2 if tc and K >= 64 and parts * rank <= 512 and (2 if woven else 1) * rank <= 256 else 0}
         self._err = device_error_word(a.device).data_ptr()
         self._index = a.get_device()
 
@@ -543,11 +545,11 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, rows: Ad
         if out.shape != base.shape or out.dtype != dtype:
             raise InvalidInput("adapter_add: out must be like base")
     xp = x.data_ptr()
-    form = 1 if rows.tile == 16 and bank._tensor_cores and (xp | ld_x * 2) % 16 == 0 else 0
+    form = bank._form[rows.tile] if (xp | ld_x * 2) % 16 == 0 else 0
     lib = native.lib()
     low = 0
-    if form == 0:
-        scratch = _new((lib.rfx_adapter_low_floats(bank._ptr, R, form),), torch.float32, x.device)
+    if form != 1:
+        scratch = _new((lib.rfx_adapter_low_floats(bank._ptr, R, rows.n_tiles, form),), torch.float32, x.device)
         low = scratch.data_ptr()
     st = lib.rfx_adapter_add(
         bank._ptr, rows.order_ptr, rows.tiles_ptr, rows.n_tiles, rows.tile, base.data_ptr(), ld_base, out.data_ptr(),
