@@ -296,7 +296,7 @@ extern "C" int rfx_adapter_add(const AdapterBank* k, const int* order, const int
     cudaStream_t s = (cudaStream_t)stream;
     if (form == 1) return k->dt == RFX_DT_BF16 && step_takes(p) ? step_form(p, dt_out, s) : RFX_ERR_UNSUPPORTED;
     if (form == 2 && low)
-        return k->dt == RFX_DT_BF16 && prompt_takes(p) ? prompt_form(p, dt_out, err, s) : RFX_ERR_UNSUPPORTED;
+        return k->dt == RFX_DT_BF16 && prompt_takes(p, dt_out) ? prompt_form(p, dt_out, err, s) : RFX_ERR_UNSUPPORTED;
     if (form != 0 || !low) return RFX_ERR_BAD_ARG;
     if (k->dt == RFX_DT_F32) return fma_form<float, float>(p, s);
     if (dt_out == RFX_DT_F32) return fma_form<__nv_bfloat16, float>(p, s);

@@ -229,6 +229,25 @@ __device__ __forceinline__ void tmem_loaded_8(uint32_t* r) {
                  : "memory");
 }
 
+// 16 lanes x 32 columns, in the layout of an m16n8 accumulator, four of them side by side: thread (g, t) = (lane / 4,
+// lane % 4) gets rows g and g + 8 of columns 8 i + 2 t and the next in registers 4 i .. 4 i + 3 (rows g, g, g + 8, g + 8).
+__device__ __forceinline__ void tmem_ld_frag4_nowait(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32"
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// Two of them.
+__device__ __forceinline__ void tmem_ld_frag2_nowait(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        : "r"(taddr));
+}
+
 // The same load without the wait: issue several, then tmem_ld_wait_16 with one's registers, tmem_loaded_16 with the others'.
 __device__ __forceinline__ void tmem_ld_16_nowait(uint32_t taddr, uint32_t* r) {
     asm volatile(

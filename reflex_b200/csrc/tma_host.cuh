@@ -32,12 +32,12 @@ inline EncodeTiledFn encode_fn() {
 // A [rows, cols] row-major bfloat16 matrix read in boxes of `box_rows` rows x 64
 // columns (128 bytes) with the 128-byte swizzle: 16-byte chunk c of row r lands
 // at chunk c ^ (r & 7) of that row's 128 bytes.  `cols` a multiple of 8, `base`
-// 16-byte aligned.
-inline bool make_map_rows64(CUtensorMap* map, const void* base, long long rows, int cols, int box_rows) {
+// 16-byte aligned.  `ld` (a multiple of 8): the elements from one row to the next, `cols` where it is 0.
+inline bool make_map_rows64(CUtensorMap* map, const void* base, long long rows, int cols, int box_rows, long long ld = 0) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
+    cuuint64_t strides[1] = {(cuuint64_t)(ld ? ld : cols) * 2};
     cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,

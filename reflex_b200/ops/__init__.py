@@ -488,10 +488,12 @@ class AdapterBank:
         ints[:8 + parts] = [n, K, lda, N, rank, parts, int(self.woven), dt_code(a.dtype)] + [
             sum(cols[:i + 1]) for i in range(parts)]
         self._ptr = ctypes.addressof(self._desc)
-        # which tiles the tensor cores take (bfloat16 rows on 16 bytes): of 16 rows, of 128 rows
+        # which tiles the tensor cores take (bfloat16 rows on 16 bytes), for a base in bfloat16 and in 32-bit
         tc = a.dtype == torch.bfloat16 and K % 8 == 0 and (a.data_ptr() | b.data_ptr()) % 16 == 0
-        self._form = {16: 1 if tc else 0,
-                      128: 2 if tc and K >= 64 and parts * rank <= 512 and (2 if woven else 1) * rank <= 256 else 0}
+        blocks = 99 if K < 64 or parts * rank > 512 else (2 if woven else 1) * ((rank + 63) // 64)
+        self._form = {(16, torch.float32): 1 if tc else 0, (16, torch.bfloat16): 1 if tc else 0,
+                      (128, torch.float32): 2 if tc and blocks <= 3 else 0,
+                      (128, torch.bfloat16): 2 if tc and blocks <= 4 else 0}
         self._err = device_error_word(a.device).data_ptr()
         self._index = a.get_device()
 
@@ -545,7 +547,7 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, rows: Ad
         if out.shape != base.shape or out.dtype != dtype:
             raise InvalidInput("adapter_add: out must be like base")
     xp = x.data_ptr()
-    form = bank._form[rows.tile] if (xp | ld_x * 2) % 16 == 0 else 0
+    form = bank._form[rows.tile, dtype] if (xp | ld_x * 2) % 16 == 0 else 0
     lib = native.lib()
     low = 0
     if form != 1:
