@@ -270,9 +270,9 @@ struct AdapterBank {
 
 // Floats of scratch that rfx_adapter_add needs in a form: 0 the products in 32-bit multiply-adds, 1 tiles of
 // 16 rows and 2 tiles of 128 rows on the tensor cores.
-extern "C" long long rfx_adapter_low_floats(const AdapterBank* k, int R, int max_tiles, int form) {
-    if (R <= 0 || max_tiles <= 0 || !k || k->K <= 0 || form == 1) return 0;
-    if (form == 2) return prompt_low_floats(R, k->K, k->parts * k->rank, max_tiles);
+extern "C" long long rfx_adapter_low_floats(const AdapterBank* k, int R, int form) {
+    if (R <= 0 || !k || k->K <= 0 || form == 1) return 0;
+    if (form == 2) return prompt_low_floats(R, k->parts * k->rank);
     return (long long)k_pieces(k->K) * R * k->parts * k->rank;
 }
 

@@ -56,7 +56,7 @@ bool step_takes(const Args& p);
 int step_form(const Args& p, int dt_out, cudaStream_t s);
 // tiles of 128 rows, bfloat16 (adapters_prompt.cu)
 bool prompt_takes(const Args& p, int dt_out);
-long long prompt_low_floats(int R, int K, int W, int max_tiles);
+long long prompt_low_floats(int R, int W);
 int prompt_form(const Args& p, int dt_out, int* err, cudaStream_t s);
 
 }  // namespace adapters

@@ -492,7 +492,7 @@ class AdapterBank:
         tc = a.dtype == torch.bfloat16 and K % 8 == 0 and (a.data_ptr() | b.data_ptr()) % 16 == 0
         blocks = 99 if K < 64 or parts * rank > 512 else (2 if woven else 1) * ((rank + 63) // 64)
         self._form = {(16, torch.float32): 1 if tc else 0, (16, torch.bfloat16): 1 if tc else 0,
-                      (128, torch.float32): 2 if tc and blocks <= 3 else 0,
+                      (128, torch.float32): 2 if tc and blocks <= 2 else 0,
                       (128, torch.bfloat16): 2 if tc and blocks <= 4 else 0}
         self._err = device_error_word(a.device).data_ptr()
         self._index = a.get_device()
@@ -551,7 +551,7 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, rows: Ad
     lib = native.lib()
     low = 0
     if form != 1:
-        scratch = _new((lib.rfx_adapter_low_floats(bank._ptr, R, rows.n_tiles, form),), torch.float32, x.device)
+        scratch = _new((lib.rfx_adapter_low_floats(bank._ptr, R, form),), torch.float32, x.device)
         low = scratch.data_ptr()
     st = lib.rfx_adapter_add(
         bank._ptr, rows.order_ptr, rows.tiles_ptr, rows.n_tiles, rows.tile, base.data_ptr(), ld_base, out.data_ptr(),

@@ -261,7 +261,7 @@ def lib() -> ctypes.CDLL:
         handle.rfx_delta_rule_chunk_floats.restype = c_longlong
         handle.rfx_sm_count.argtypes = []
         handle.rfx_sm_count.restype = c_int
-        handle.rfx_adapter_low_floats.argtypes = [c_void_p, c_int, c_int, c_int]
+        handle.rfx_adapter_low_floats.argtypes = [c_void_p, c_int, c_int]
         handle.rfx_adapter_low_floats.restype = c_longlong
         handle.rfx_sample_work_bytes.argtypes = [c_int, c_int]
         handle.rfx_sample_work_bytes.restype = c_longlong
