@@ -268,6 +268,17 @@ struct AdapterBank {
     int ends[MAX_PARTS];  // a part's last column and one
 };
 
+// The form that takes tiles of so many rows where x's lie on 16 bytes (0 takes them all): what rfx_adapter_add is
+// given as `form`.
+extern "C" int rfx_adapter_form(const AdapterBank* k, int tile, int dt_out) {
+    if (!k || k->dt != RFX_DT_BF16 || k->K <= 0 || k->rank <= 0 || k->parts <= 0 || k->parts > MAX_PARTS) return 0;
+    Args p{nullptr, nullptr, nullptr, k->a, k->b, k->scale, k->ranks, nullptr, nullptr, nullptr, 0, 0, 0, k->n, 1, k->K,
+           k->lda, k->N, k->rank, 1, tile, {}};
+    p.parts.n = k->parts;
+    p.parts.woven = k->woven;
+    return step_takes(p) ? 1 : prompt_takes(p, dt_out) ? 2 : 0;
+}
+
 // Floats of scratch that rfx_adapter_add needs in a form: 0 the products in 32-bit multiply-adds, 1 tiles of
 // 16 rows and 2 tiles of 128 rows on the tensor cores.
 extern "C" long long rfx_adapter_low_floats(const AdapterBank* k, int R, int form) {

@@ -1,15 +1,15 @@
 // The adapters of a step's requests, a row or a few each: tiles of at most 16 rows, bfloat16, one launch.
 //
 // A thread-block cluster takes a tile and both products.  Each of its eight CTAs multiplies the tile's rows
-// with A over an eighth of K on the tensor cores (m16n8k16: 16 rows, 8 rank rows), its warps over every eighth
-// 32 of that; the partial sums meet in shared memory and, over the cluster, in distributed shared memory, in
-// rank order; then each CTA multiplies the low-rank rows with its share of B's columns and adds the base.
-// Nothing but the result goes back to memory, and there is one launch where two would have to follow one another.
+// with A over an eighth of K on the tensor cores (m16n8k16: 16 rows, 8 rank rows), a warp every eighth 8 rank rows;
+// the partial sums meet in distributed shared memory, in rank order; then each CTA multiplies the low-rank rows
+// with its share of B's columns and adds the base.  Nothing but the result goes back to memory, and there is
+// one launch where two would have to follow one another.
 //
-// It is latency and the adapters' bytes that count (an adapter of rank 16 beside 4,096 x 6,144: 0.6 MB): operands
-// come from memory straight into fragments by 16- and 8-byte loads, with k permuted alike on both sides so
-// that a lane's elements lie side by side, and a warp's first columns of B and of the base are on their way
-// before the cluster meets.
+// It is latency and the adapters' bytes that count (an adapter of rank 16 beside 4,096 x 6,144: 0.6 MB).  So a warp
+// has 6 KB of A on their way, in a ring of shared memory of which every lane reads what it brought itself (no
+// barrier), k permuted alike on both sides so that a lane's elements lie side by side; B's columns are asked
+// for ahead, and a warp's first ones and their base are loaded before the cluster meets.
 //
 // The low-rank rows are kept in 32 bits and go into the second product as three bfloat16 parts (24 bits).
 // How K is cut depends on K alone, and a row's sums on nothing else in the tile, so a row has the same bits
@@ -27,19 +27,24 @@ using namespace rfx;
 using namespace adapters;
 
 constexpr int CLUSTER = 8, THREADS = 256, WARPS = THREADS / 32, TILE = 16;
-constexpr int CHUNK = 8;                    // tiles of 8 rank rows that a warp sums at a time
-constexpr int RED_LD = CHUNK * 8 + 4;
+constexpr int RING = 3, BATCH = 4;          // a warp's batches of A under way, of 8 rank rows by 4 times 32 of K
 constexpr int GROUP = 32;                   // columns a warp makes at a time
-constexpr int AHEAD = 4;                    // steps of 16 along the rank whose B is loaded before the cluster meets
+constexpr int AHEAD = 2;                    // steps of 16 along the rank whose B is loaded before the cluster meets
 
-__host__ __device__ inline int k_slice(int K) { return ((K + CLUSTER - 1) / CLUSTER + 31) / 32 * 32; }
-// floats of the partial rows, and the three parts' bfloat16s
-inline size_t step_smem(int W) {
-    return (size_t)WARPS * TILE * RED_LD * 4 + (size_t)TILE * W * 4 + (size_t)3 * TILE * (W + 8) * 2;
+// (in whole batches of 128)
+__host__ __device__ inline int k_slice(int K) { return ((K + CLUSTER - 1) / CLUSTER + 127) / 128 * 128; }
+// the warps' pieces of A, the rows of x, the partial rows, and the three parts' bfloat16s
+inline size_t step_smem(int W, int K) {
+    return (size_t)WARPS * RING * BATCH * 512 + (size_t)TILE * (k_slice(K) + 8) * 2 + (size_t)TILE * W * 4 +
+           (size_t)3 * TILE * (W + 8) * 2;
 }
 
-__device__ __forceinline__ uint4 load16(const __nv_bfloat16* p, bool valid) {
-    return valid ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
 }
 
 template <typename TO>
@@ -49,13 +54,14 @@ __device__ __forceinline__ void load8(const TO* p, float (&v)[8]) {
 }
 
 template <typename TO>
-__global__ void __launch_bounds__(THREADS) adapter_step_kernel(const Args p, int groups, int vec) {
+__global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, int groups, int vec) {
     extern __shared__ __align__(16) uint8_t dynamic[];
     __shared__ int rows[TILE];
     cg::cluster_group cluster = cg::this_cluster();
-    const int W = p.parts.n * p.rank, LDV = W + 8;
-    float* red = reinterpret_cast<float*>(dynamic);                                       // [WARPS][TILE][RED_LD]
-    float* part_v = red + WARPS * TILE * RED_LD;                                          // [TILE][W]
+    const int W = p.parts.n * p.rank, LDV = W + 8, slice = k_slice(p.K), LDX = slice + 8;
+    uint8_t* ring = dynamic;                                                              // [WARPS][RING][BATCH][lane]
+    __nv_bfloat16* xs = reinterpret_cast<__nv_bfloat16*>(ring + WARPS * RING * BATCH * 512);  // [TILE][LDX]
+    float* part_v = reinterpret_cast<float*>(xs + TILE * LDX);                            // [TILE][W]
     __nv_bfloat16* vs = reinterpret_cast<__nv_bfloat16*>(part_v + TILE * W);              // [3][TILE][LDV]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     pdl_prologue();
@@ -64,10 +70,42 @@ __global__ void __launch_bounds__(THREADS) adapter_step_kernel(const Args p, int
     const bool none = tile.adapter >= p.n;
     if (none && p.out == p.base) return;
     const int count = min(tile.count, TILE), c = cluster.block_rank();
-    if (tid < TILE) rows[tid] = p.order[tile.place + min(tid, count - 1)];
     const int rank = none ? 0 : p.rank_of(tile.adapter);
     const int per = (rank + 7) / 8, steps = (rank + 15) / 16, tiles = per * p.parts.n;
+    // ---- a warp's first pieces of A: tiles of 8 rank rows n = warp, warp + 8, ..., 128 of K at a time; a lane brings,
+    // and reads, its own 16 bytes of each 32
+    const int k0 = c * slice, k1 = min(p.K, k0 + slice), blocks = k0 < k1 ? (k1 - k0 + 31) / 32 : 0;
+    const __nv_bfloat16* a = (const __nv_bfloat16*)p.a + (size_t)tile.adapter * W * p.lda;
+    const uint32_t my_ring = attn::smem_u32(ring) + warp * RING * BATCH * 512 + lane * 16;
+    int next_n = blocks ? warp : tiles, next_b = 0, next_slot = 0;
+    auto bring = [&]() {
+        if (next_n < tiles) {
+            const int s = next_n / per, row = s * p.rank + (next_n - s * per) * 8 + g;
+            const __nv_bfloat16* src = a + (size_t)row * p.lda + k0 + next_b * 32 + t * 8;
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const int bytes = k0 + (next_b + j) * 32 + t * 8 < k1 ? 16 : 0;  // (zeros beyond)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(my_ring + (next_slot * BATCH + j) * 512),
+                             "l"(bytes ? src + j * 32 : a), "r"(bytes)
+                             : "memory");
+            }
+            if ((next_b += BATCH) >= blocks) next_b = 0, next_n += WARPS;
+            if (++next_slot == RING) next_slot = 0;
+        }
+        attn::cp_async_commit();
+    };
+    for (int i = 0; i < RING - 1; ++i) bring();
+    if (tid < TILE) rows[tid] = p.order[tile.place + min(tid, count - 1)];
     __syncthreads();
+    // ---- x's rows over this CTA's slice of K
+    if (!none) {
+        const __nv_bfloat16* x = (const __nv_bfloat16*)p.x;
+        const int padded = (blocks + BATCH - 1) / BATCH * BATCH * 32;
+        for (int r = warp; r < count; r += WARPS)
+            for (int k = lane * 8; k < padded; k += 256)
+                attn::cp_async_16(xs + r * LDX + k, k0 + k < k1 ? x + (size_t)rows[r] * p.ld_x + k0 + k : x, k0 + k < k1);
+    }
+    attn::cp_async_commit();
 
     // a warp's columns: groups of 32 from the start of a part (woven: of the whole), lane (g, t) has columns
     // 8 t .. 8 t + 7 of rows g and g + 8
@@ -115,55 +153,47 @@ __global__ void __launch_bounds__(THREADS) adapter_step_kernel(const Args p, int
                 for (int j = 0; j < 4; ++j) ahead[s][j] = load_b(col, end, s, j);
         load_base(col, end, g, base_lo);
         load_base(col, end, g + 8, base_hi);
+        // B's columns of this warp are asked for, and come from L2 when their turn has come
+        if (!none)
+            for (int q = group; q < groups; q += stride) {
+                int col_q, end_q, part_q;
+                locate(q, col_q, end_q, part_q);
+                const int n = min(GROUP, end_q - col_q) * p.rank;  // (one stretch of memory)
+                for (int i = lane * 64; i < n; i += 32 * 64) prefetch_l2(b + (size_t)col_q * p.rank + i);
+            }
     }
 
     if (!none) {
         // ---- the low-rank rows over this CTA's slice of K
-        const __nv_bfloat16* a = (const __nv_bfloat16*)p.a + (size_t)tile.adapter * W * p.lda;
-        const __nv_bfloat16* x = (const __nv_bfloat16*)p.x;
-        const __nv_bfloat16 *x0 = x + (size_t)rows[g] * p.ld_x, *x1 = x + (size_t)rows[g + 8] * p.ld_x;
-        const int k0 = c * k_slice(p.K), k1 = min(p.K, k0 + k_slice(p.K));
         for (int i = tid; i < 3 * TILE * LDV / 2; i += THREADS) reinterpret_cast<uint32_t*>(vs)[i] = 0u;
-        for (int n0 = 0; n0 < tiles; n0 += CHUNK) {
-            const int here = min(CHUNK, tiles - n0);
-            float acc[CHUNK][4] = {};
-            const __nv_bfloat16* a_row[CHUNK];
+        attn::cp_async_wait<0>();
+        __syncthreads();  // x is there
+        const uint32_t x_at = attn::smem_u32(xs) + (g * LDX + t * 8) * 2;
+        int slot = 0;
+        for (int n = warp; n < tiles; n += WARPS) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < blocks; i += BATCH) {
+                bring();
+                attn::cp_async_wait<RING - 1>();
+                uint4 w[BATCH], xa[BATCH], xb[BATCH];
 #pragma unroll
-            for (int i = 0; i < CHUNK; ++i) {
-                const int n = n0 + min(i, here - 1), s = n / per;
-                a_row[i] = a + (size_t)(s * p.rank + (n - s * per) * 8 + g) * p.lda;
-            }
-#pragma unroll 2
-            for (int k = k0 + warp * 32; k < k1; k += WARPS * 32) {
-                const int kt = k + t * 8;
-                const bool in = kt < k1;
-                const uint4 xa = load16(x0 + kt, in && g < count), xb = load16(x1 + kt, in && g + 8 < count);
-                uint4 w[CHUNK];
+                for (int j = 0; j < BATCH; ++j) {
+                    w[j] = lds16(my_ring + (slot * BATCH + j) * 512);
+                    xa[j] = lds16(x_at + (i + j) * 64);
+                    xb[j] = lds16(x_at + 8 * LDX * 2 + (i + j) * 64);
+                }
+                if (++slot == RING) slot = 0;
 #pragma unroll
-                for (int i = 0; i < CHUNK; ++i) w[i] = load16(a_row[i] + kt, in && i < here);
-                const uint32_t f0[4] = {xa.x, xb.x, xa.y, xb.y}, f1[4] = {xa.z, xb.z, xa.w, xb.w};
-#pragma unroll
-                for (int i = 0; i < CHUNK; ++i) {
-                    attn::mma_bf16(acc[i], f0, w[i].x, w[i].y);
-                    attn::mma_bf16(acc[i], f1, w[i].z, w[i].w);
+                for (int j = 0; j < BATCH; ++j) {
+                    const uint32_t f0[4] = {xa[j].x, xb[j].x, xa[j].y, xb[j].y}, f1[4] = {xa[j].z, xb[j].z, xa[j].w, xb[j].w};
+                    attn::mma_bf16(acc, f0, w[j].x, w[j].y);
+                    attn::mma_bf16(acc, f1, w[j].z, w[j].w);
                 }
             }
-            __syncthreads();  // the sums of the chunk before have been read
-            float* mine = red + warp * TILE * RED_LD;
-#pragma unroll
-            for (int i = 0; i < CHUNK; ++i) {
-                store2(mine + g * RED_LD + i * 8 + t * 2, acc[i][0], acc[i][1]);
-                store2(mine + (g + 8) * RED_LD + i * 8 + t * 2, acc[i][2], acc[i][3]);
-            }
-            __syncthreads();
-            for (int i = tid; i < count * CHUNK * 8; i += THREADS) {
-                const int r = i / (CHUNK * 8), n = i % (CHUNK * 8);
-                float v = 0.f;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) v += red[(w * TILE + r) * RED_LD + n];
-                if (n < here * 8) part_v[r * W + n0 * 8 + n] = v;
-            }
+            store2(part_v + g * W + n * 8 + t * 2, acc[0], acc[1]);
+            store2(part_v + (g + 8) * W + n * 8 + t * 2, acc[2], acc[3]);
         }
+        attn::cp_async_wait<0>();
         cluster.sync();
         // ---- the cluster's sums, in three parts of bfloat16
         for (int i = tid; i < count * tiles * 8; i += THREADS) {
@@ -252,7 +282,7 @@ int go(const Args& p, cudaStream_t s) {
     int share = (sm_count() + CLUSTER * p.max_tiles - 1) / (CLUSTER * p.max_tiles);
     const int most = (groups + CLUSTER * WARPS - 1) / (CLUSTER * WARPS);
     if (share > most) share = most;
-    const size_t smem = step_smem(W);
+    const size_t smem = step_smem(W, p.K);
     // rows of base and out by 16 bytes
     const size_t align = (size_t)p.base | (size_t)p.out | (size_t)(p.ld_base * sizeof(TO)) | (size_t)(p.ld_out * sizeof(TO));
     const int vec = (align & 15) == 0;
@@ -271,7 +301,7 @@ namespace adapters {
 bool step_takes(const Args& p) {
     const size_t align = (size_t)p.x | (size_t)p.a | (size_t)p.b | (size_t)(p.ld_x * 2) | (size_t)(p.lda * 2);
     return p.tile == TILE && (align & 15) == 0 && p.K % 8 == 0 && p.rank % 16 == 0 && p.max_tiles <= 65535 &&
-           step_smem(p.parts.n * p.rank) <= 220 * 1024;
+           step_smem(p.parts.n * p.rank, p.K) <= 220 * 1024;
 }
 
 int step_form(const Args& p, int dt_out, cudaStream_t s) {

@@ -488,12 +488,10 @@ class AdapterBank:
         ints[:8 + parts] = [n, K, lda, N, rank, parts, int(self.woven), dt_code(a.dtype)] + [
             sum(cols[:i + 1]) for i in range(parts)]
         self._ptr = ctypes.addressof(self._desc)
-        # which tiles the tensor cores take (bfloat16 rows on 16 bytes), for a base in bfloat16 and in 32-bit
-        tc = a.dtype == torch.bfloat16 and K % 8 == 0 and (a.data_ptr() | b.data_ptr()) % 16 == 0
-        blocks = 99 if K < 64 or parts * rank > 512 else (2 if woven else 1) * ((rank + 63) // 64)
-        self._form = {(16, torch.float32): 1 if tc else 0, (16, torch.bfloat16): 1 if tc else 0,
-                      (128, torch.float32): 2 if tc and blocks <= 2 else 0,
-                      (128, torch.bfloat16): 2 if tc and blocks <= 4 else 0}
+        # the kernels' forms (csrc/adapters.cu) by tile and base
+        form = native.lib().rfx_adapter_form
+        self._form = {(tile, dt): form(self._ptr, tile, dt_code(dt))
+                      for tile in (16, 128) for dt in (torch.float32, torch.bfloat16)}
         self._err = device_error_word(a.device).data_ptr()
         self._index = a.get_device()
 
