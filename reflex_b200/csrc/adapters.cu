@@ -141,11 +141,23 @@ constexpr int LOW_SPLITS = 8, ROWS = 32, COLS = 32, BK = 32, OUT_COLS = 64;
 __host__ __device__ inline int k_piece(int K) { return ((K + LOW_SPLITS - 1) / LOW_SPLITS + BK - 1) / BK * BK; }
 __host__ __device__ inline int k_pieces(int K) { return (K + k_piece(K) - 1) / k_piece(K); }
 
-// low[piece][place][part * rank + i]: 32 rows x 32 rank rows a block, four sums a thread
+// Four neighbours of a row's first `left`, zeros beyond; `whole`: the row's fours lie on their own size.
 template <typename T>
-__global__ void __launch_bounds__(256) adapter_low_kernel(const Args p) {
-    __shared__ float xs[ROWS][BK + 1], as[COLS][BK + 1];
-    __shared__ int rows[ROWS];
+__device__ __forceinline__ float4 four(const T* p, int left, bool whole) {
+    if (whole && left >= 4) return load4(p);
+    return make_float4(left > 0 ? ld(p, 0) : 0.f, left > 1 ? ld(p, 1) : 0.f, left > 2 ? ld(p, 2) : 0.f,
+                       left > 3 ? ld(p, 3) : 0.f);
+}
+__device__ __forceinline__ void fma4(float& s, const float4& a, const float4& b) {
+    s = fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
+}
+
+// low[piece][place][part * rank + i]: 32 rows x 32 rank rows a block, four sums a thread; the next 32 of K are on
+// their way while these are multiplied.
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_low_kernel(const Args p, int x_whole, int a_whole) {
+    constexpr int LD = BK + 4;
+    __shared__ __align__(16) float xs[2][ROWS][LD], as[2][COLS][LD];
     pdl_prologue();
     const int subs = (p.tile + ROWS - 1) / ROWS;
     const Tile t = load_tile(p.tiles, blockIdx.x / subs);
@@ -153,25 +165,27 @@ __global__ void __launch_bounds__(256) adapter_low_kernel(const Args p) {
     if (t.adapter < 0 || t.adapter >= p.n || sub >= t.count) return;
     const int here = min(ROWS, t.count - sub), w0 = blockIdx.y * COLS, rank = p.rank_of(t.adapter);
     const int k0 = blockIdx.z * k_piece(p.K), k1 = min(p.K, k0 + k_piece(p.K));
-    if (threadIdx.x < ROWS) rows[threadIdx.x] = p.order[t.place + sub + min((int)threadIdx.x, here - 1)];
-    __syncthreads();
-    const T* x = (const T*)p.x;
-    const T* a = (const T*)p.a + (size_t)t.adapter * W * p.lda;
+    // what this thread brings: four of K of a row of x and of a rank row
+    const int row = threadIdx.x >> 3, k4 = (threadIdx.x & 7) * 4, w = w0 + row;
+    const T* x = (const T*)p.x + (size_t)p.order[t.place + sub + min(row, here - 1)] * p.ld_x;
+    const T* a = (const T*)p.a + ((size_t)t.adapter * W + min(w, W - 1)) * p.lda;
+    const bool a_on = w < W && w % p.rank < rank;
+    auto load_x = [&](int k) { return four(x + k + k4, k1 - k - k4, x_whole); };
+    auto load_a = [&](int k) { return four(a + k + k4, a_on ? k1 - k - k4 : 0, a_whole); };
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = k0; k < k1; k += BK) {
-        const bool in = k + tx < k1;
-#pragma unroll
-        for (int i = ty; i < ROWS; i += 8) xs[i][tx] = in && i < here ? ld(x, (size_t)rows[i] * p.ld_x + k + tx) : 0.f;
-#pragma unroll
-        for (int i = ty; i < COLS; i += 8)
-            as[i][tx] = in && w0 + i < W && (w0 + i) % p.rank < rank ? ld(a, (size_t)(w0 + i) * p.lda + k + tx) : 0.f;
+    float4 nx = load_x(k0), na = load_a(k0);
+    for (int k = k0, s = 0; k < k1; k += BK, s ^= 1) {
+        store4(&xs[s][row][k4], nx);
+        store4(&as[s][row][k4], na);
         __syncthreads();
-        const int most = min(BK, k1 - k);
-        for (int kk = 0; kk < most; ++kk)
+        if (k + BK < k1) nx = load_x(k + BK), na = load_a(k + BK);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = fmaf(xs[ty * 4 + j][kk], as[tx][kk], acc[j]);
-        __syncthreads();
+        for (int kk = 0; kk < BK; kk += 4) {
+            const float4 av = load4(&as[s][tx][kk]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) fma4(acc[j], load4(&xs[s][ty * 4 + j][kk]), av);
+        }
     }
     if (w0 + tx < W)
 #pragma unroll
@@ -182,50 +196,63 @@ __global__ void __launch_bounds__(256) adapter_low_kernel(const Args p) {
 
 // 32 rows x 64 columns a block, eight rows a thread
 template <typename T, typename TO>
-__global__ void __launch_bounds__(256) adapter_up_kernel(const Args p) {
-    extern __shared__ float vs[];  // [ROWS][W]
+__global__ void __launch_bounds__(256) adapter_up_kernel(const Args p, int b_whole) {
+    extern __shared__ __align__(16) float vs[];  // [ROWS][parts][rank in fours]
     __shared__ int rows[ROWS];
     pdl_prologue();
     const int subs = (p.tile + ROWS - 1) / ROWS;
     const Tile t = load_tile(p.tiles, blockIdx.x / subs);
-    const int sub = blockIdx.x % subs * ROWS, W = p.parts.n * p.rank;
+    const int sub = blockIdx.x % subs * ROWS, W = p.parts.n * p.rank, wide = (p.rank + 3) / 4 * 4, LD = p.parts.n * wide;
     if (t.adapter < 0 || sub >= t.count) return;
     const bool none = t.adapter >= p.n;
     if (none && p.out == p.base) return;
     const int here = min(ROWS, t.count - sub);
     if (threadIdx.x < ROWS) rows[threadIdx.x] = p.order[t.place + sub + min((int)threadIdx.x, here - 1)];
-    const int pieces = k_pieces(p.K);
-    if (!none)
-        for (int i = threadIdx.x; i < here * W; i += 256) {
-            float v = 0.f;
-            for (int s = 0; s < pieces; ++s) v += p.low[((size_t)s * p.R + t.place + sub) * W + i];
-            vs[i] = v;
-        }
     __syncthreads();
-    const int c = blockIdx.y * OUT_COLS + (threadIdx.x & 63), r0 = (threadIdx.x >> 6) * 8;
-    if (c >= p.N) return;
+    const int c = blockIdx.y * OUT_COLS + (threadIdx.x & 63), r0 = (threadIdx.x >> 6) * 8, r1 = min(here, r0 + 8);
     const TO* base = (const TO*)p.base;
     TO* out = (TO*)p.out;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (c < p.N && r0 + j < r1) y[j] = ld(base, (size_t)rows[r0 + j] * p.ld_base + c);
     float acc[8] = {};
     float scale = 0.f;
     if (!none) {
-        const int rank = p.rank_of(t.adapter);
-        const T* b = (const T*)p.b + ((size_t)t.adapter * p.N + c) * p.rank;
-        const float* v = vs + p.parts.part_of(c) * p.rank;
-        scale = p.scale[t.adapter];
-        for (int i = 0; i < rank; ++i) {
-            const float bi = ld(b, i);
+        const int pieces = k_pieces(p.K);
+        for (int i = threadIdx.x; i < here * LD; i += 256) {
+            const int r = i / LD, q = (i - r * LD) / wide, k = i - r * LD - q * wide;
+            float v = 0.f;
+            if (k < p.rank) {
+                const float* src = p.low + ((size_t)t.place + sub + r) * W + q * p.rank + k;
+                float d[LOW_SPLITS];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (r0 + j < here) acc[j] = fmaf(v[(r0 + j) * W + i], bi, acc[j]);
+                for (int s = 0; s < LOW_SPLITS; ++s) d[s] = s < pieces ? src[(size_t)s * p.R * W] : 0.f;
+#pragma unroll
+                for (int s = 0; s < LOW_SPLITS; ++s)
+                    if (s < pieces) v += d[s];
+            }
+            vs[i] = v;
+        }
+        __syncthreads();
+        if (c < p.N) {
+            const int rank = p.rank_of(t.adapter);
+            const T* b = (const T*)p.b + ((size_t)t.adapter * p.N + c) * p.rank;
+            const float* v = vs + p.parts.part_of(c) * wide + r0 * LD;
+            scale = p.scale[t.adapter];
+#pragma unroll 2
+            for (int i = 0; i < rank; i += 4) {
+                const float4 bi = four(b + i, p.rank - i, b_whole);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (r0 + j < r1) fma4(acc[j], load4(v + j * LD + i), bi);
+            }
         }
     }
+    if (c < p.N)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (r0 + j < here) {
-            const float y = ld(base, (size_t)rows[r0 + j] * p.ld_base + c);
-            st(out, (size_t)rows[r0 + j] * p.ld_out + c, none ? y : fmaf(scale, acc[j], y));
-        }
+        for (int j = 0; j < 8; ++j)
+            if (r0 + j < r1) st(out, (size_t)rows[r0 + j] * p.ld_out + c, none ? y[j] : fmaf(scale, acc[j], y[j]));
 }
 
 template <typename T, typename TO>
@@ -234,12 +261,17 @@ int fma_form(const Args& p, cudaStream_t s) {
     const long long blocks = (long long)p.max_tiles * subs;
     if (blocks > 0x7fffffffLL || (p.N + OUT_COLS - 1) / OUT_COLS > 65535 || (W + COLS - 1) / COLS > 65535)
         return RFX_ERR_UNSUPPORTED;
-    const size_t smem = (size_t)ROWS * W * sizeof(float);
+    const size_t smem = (size_t)ROWS * p.parts.n * ((p.rank + 3) / 4 * 4) * sizeof(float);
+    // rows that can be read by fours
+    const size_t mask = 4 * sizeof(T) - 1;
+    const int x_whole = (((size_t)p.x | (size_t)(p.ld_x * sizeof(T))) & mask) == 0;
+    const int a_whole = (((size_t)p.a | (size_t)(p.lda * sizeof(T))) & mask) == 0;
+    const int b_whole = (((size_t)p.b | (size_t)(p.rank * sizeof(T))) & mask) == 0;
     static SmemLimit limit;
     cudaError_t e = limit.raise(adapter_up_kernel<T, TO>, smem);
     if (e != cudaSuccess) return (int)e;
-    RFX_LAUNCH(adapter_low_kernel<T>, dim3((unsigned)blocks, (W + COLS - 1) / COLS, k_pieces(p.K)), 256, 0, s, p);
-    RFX_LAUNCH((adapter_up_kernel<T, TO>), dim3((unsigned)blocks, (p.N + OUT_COLS - 1) / OUT_COLS), 256, smem, s, p);
+    RFX_LAUNCH(adapter_low_kernel<T>, dim3((unsigned)blocks, (W + COLS - 1) / COLS, k_pieces(p.K)), 256, 0, s, p, x_whole, a_whole);
+    RFX_LAUNCH((adapter_up_kernel<T, TO>), dim3((unsigned)blocks, (p.N + OUT_COLS - 1) / OUT_COLS), 256, smem, s, p, b_whole);
     return 0;
 }
 

@@ -153,13 +153,14 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, 
                 for (int j = 0; j < 4; ++j) ahead[s][j] = load_b(col, end, s, j);
         load_base(col, end, g, base_lo);
         load_base(col, end, g + 8, base_hi);
-        // B's columns of this warp are asked for, and come from L2 when their turn has come
+        // this warp's columns of B and of base are asked for, and come from L2 when their turn has come
         if (!none)
             for (int q = group; q < groups; q += stride) {
                 int col_q, end_q, part_q;
                 locate(q, col_q, end_q, part_q);
                 const int n = min(GROUP, end_q - col_q) * p.rank;  // (one stretch of memory)
                 for (int i = lane * 64; i < n; i += 32 * 64) prefetch_l2(b + (size_t)col_q * p.rank + i);
+                if (q != group && lane < count) prefetch_l2(base + (size_t)rows[lane] * p.ld_base + col_q);
             }
     }
 
@@ -278,8 +279,9 @@ int go(const Args& p, cudaStream_t s) {
         groups += (p.parts.end[i] - first + GROUP - 1) / GROUP;
     if (p.parts.woven) groups = (p.N + GROUP - 1) / GROUP;
     // Several clusters share a tile's columns (each makes the low-rank rows for itself, A comes from L2) until
-    // the grid holds a CTA for every SM, or every warp has one group of columns.
-    int share = (sm_count() + CLUSTER * p.max_tiles - 1) / (CLUSTER * p.max_tiles);
+    // the grid holds two CTAs for every SM, or every warp has one group of columns.
+    int share = 2 * sm_count() / (CLUSTER * p.max_tiles);
+    if (share < 1) share = 1;
     const int most = (groups + CLUSTER * WARPS - 1) / (CLUSTER * WARPS);
     if (share > most) share = most;
     const size_t smem = step_smem(W, p.K);
