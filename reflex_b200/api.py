@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
-from typing import Callable, List, Optional, Sequence, Union
+from typing import Callable, List, Mapping, Optional, Sequence, Union
 
 import torch
 
@@ -107,6 +107,7 @@ class Model:
         self.max_batch = max_batch
         self.engine = Engine(causal_lm, max_tokens=max_tokens, use_graphs=use_graphs)
         self.last_stats: Optional[GenerationStats] = None
+        self.adapter_names: List[str] = []
         # the generation loop keeps the device one step ahead of the host
         self.decode_ahead = True
 
@@ -130,27 +131,55 @@ class Model:
         sizes.update(kw)
         return cls(load_model(model_dir, _DTYPES[weights], device), **sizes)
 
+    def load_adapters(self, folders: Mapping[str, str]) -> None:
+        """Low-rank adapters by name, each from a folder (`weights.adapters`), in place of
+        those loaded before.  They stay beside the weights; prompts of one `generate`
+        call may each go through another (its `adapters`)."""
+        from .weights.adapters import read_adapter
+
+        read = [read_adapter(folder, self.spec) for folder in folders.values()]
+        self.engine.load_adapters(read)
+        self.adapter_names = list(folders)
+
+    def adapter(self, name: str) -> int:
+        """The number of a loaded adapter, as `Engine.open` takes it."""
+        if name not in self.adapter_names:
+            raise InvalidInput(f"no adapter {name!r} is loaded; loaded: {self.adapter_names}")
+        return self.adapter_names.index(name)
+
     @property
     def weights_dtype(self) -> str:
         return "bf16" if self.lm.dtype == torch.bfloat16 else "f32"
 
     # ------------------------------------------------------------------
     def generate(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]], max_new_tokens: int,
-                 sampling: Optional[SamplingParams] = None,
-                 on_token: Optional[Callable[[int, int], None]] = None):
+                 sampling: Union[SamplingParams, Sequence[SamplingParams], None] = None,
+                 on_token: Optional[Callable[[int, int], None]] = None,
+                 adapters: Union[str, Sequence[Optional[str]], None] = None):
         """Greedy by default.  One prompt (a list of ids) gives a list of ids;
         a list of prompts gives a list of lists.  Stop tokens are the model's
         end-of-sequence ids and `sampling.stop_token_ids`; the stop token is
-        kept in the output."""
-        sampling = sampling or SamplingParams()
+        kept in the output.  `sampling` may be a list with each prompt's own
+        parameters, and `adapters` the name of a loaded adapter (`load_adapters`) for
+        all prompts or a list with each prompt's (None: the model as it is): prompts
+        with different ones run in one batch."""
+        sampling = SamplingParams() if sampling is None else sampling
         single = len(prompts) > 0 and isinstance(prompts[0], int)
         plist = [list(prompts)] if single else [list(p) for p in prompts]
+        if not isinstance(sampling, SamplingParams) and len(sampling) != len(plist):
+            raise InvalidInput(f"generate: {len(plist)} prompts need as many sampling parameters, got {len(sampling)}")
         sampler = Sampler(sampling, self.lm.device)
-        stops = tuple(self.spec.eos_token_ids) + tuple(sampling.stop_token_ids)
+        own = [] if isinstance(sampling, SamplingParams) else [p.stop_token_ids for p in sampling]
+        stops = tuple(self.spec.eos_token_ids) + (() if own else tuple(sampling.stop_token_ids))
+        if adapters is not None and not isinstance(adapters, str) and len(adapters) != len(plist):
+            raise InvalidInput(f"generate: {len(plist)} prompts need as many adapters, got {len(adapters)}")
+        if adapters is not None:
+            names = [adapters] * len(plist) if isinstance(adapters, str) else adapters
+            adapters = [None if a is None else self.adapter(a) for a in names]
         stats = GenerationStats()
         out = _generate(self.engine, plist, max_new_tokens, sampler.pick, stops,
                         max_batch=self.max_batch, on_token=on_token, stats=stats,
-                        pick_async=sampler.pick_async if self.decode_ahead else None)
+                        pick_async=sampler.pick_async if self.decode_ahead else None, stops_of=own, adapters=adapters)
         self.last_stats = stats
         return out[0] if single else out
 

@@ -18,7 +18,8 @@ from typing import List, Optional
 
 USAGE = """usage: reflex <subcommand> ...
   generate <model-dir> [prompt-ids] [--max-tokens N] [--temperature F] [--top-k N] [--top-p F]
-           [--seed N] [--stop-ids a,b] [--weights bf16|f32] [--prompt-ids a,b,c]... [--json]
+           [--min-p F] [--seed N] [--stop-ids a,b] [--weights bf16|f32] [--prompt-ids a,b,c]...
+           [--adapter dir]... [--json]    (an adapter for all prompts, or one for each; -: none)
   system1  <model-dir> <prompt-ids> --candidate a,b [--candidate c]... [--temperature T]
            [--weights bf16|f32] [--json]
   check    <model-dir> <prompt-ids> [--max-tokens N] [--reference file] [--tolerance F]
@@ -95,8 +96,8 @@ def _load(path: str, weights: str, **kw):
 def cmd_generate(argv: List[str], t0: float) -> int:
     from .sampling import SamplingParams
 
-    a = Args(argv, {"--max-tokens", "--temperature", "--top-k", "--top-p", "--seed", "--weights",
-                    "--stop-ids", "--prompt-ids"}, {"--json"})
+    a = Args(argv, {"--max-tokens", "--temperature", "--top-k", "--top-p", "--min-p", "--seed", "--weights",
+                    "--stop-ids", "--prompt-ids", "--adapter"}, {"--json"})
     if not a.positional:
         fail(USAGE)
     path = a.positional[0]
@@ -108,9 +109,15 @@ def cmd_generate(argv: List[str], t0: float) -> int:
         fail("--max-tokens must be at least 1")
     sampling = SamplingParams(
         temperature=a.num("--temperature", float, 0.0), top_k=a.num("--top-k", int, None),
-        top_p=a.num("--top-p", float, None), seed=a.num("--seed", int, None),
+        top_p=a.num("--top-p", float, None), min_p=a.num("--min-p", float, None), seed=a.num("--seed", int, None),
         stop_token_ids=tuple(parse_ids(a.values.get("--stop-ids", ""))))
+    dirs = a.multi.get("--adapter", [])
+    if len(dirs) not in (0, 1, len(prompts)):
+        fail(f"--adapter is given once, or once for each of the {len(prompts)} prompts")
     model, load_ms = _load(path, resolve_weights(a.values.get("--weights")))
+    adapters = [None if d == "-" else d for d in dirs * (len(prompts) if len(dirs) == 1 else 1)] or None
+    if any(adapters or ()):
+        model.load_adapters({d: d for d in adapters if d is not None})
     first = {}
     t_gen = time.perf_counter()
 
@@ -118,7 +125,7 @@ def cmd_generate(argv: List[str], t0: float) -> int:
         if not first:
             first["ms"] = (time.perf_counter() - t0) * 1000.0
 
-    outs = model.generate(prompts, max_tokens, sampling, on_token=on_token)
+    outs = model.generate(prompts, max_tokens, sampling, on_token=on_token, adapters=adapters)
     total_ms = (time.perf_counter() - t0) * 1000.0
     gen_ms = (time.perf_counter() - t_gen) * 1000.0
     for i, ids in enumerate(outs):

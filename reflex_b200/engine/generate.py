@@ -62,8 +62,10 @@ def generate(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int,
              stop_token_ids: Sequence[int] = (), max_batch: int = 64,
              on_token: Optional[Callable[[int, int], None]] = None,
              stats: Optional[GenerationStats] = None,
-             pick_async: Optional[Callable] = None) -> List[List[int]]:
-    """Generated ids per prompt (the prompt itself is not repeated).
+             pick_async: Optional[Callable] = None, stops_of: Optional[Sequence[Sequence[int]]] = None,
+             adapters: Optional[Sequence[Optional[int]]] = None) -> List[List[int]]:
+    """Generated ids per prompt (the prompt itself is not repeated).  `stops_of`: further
+    stop tokens, prompt by prompt; `adapters`: each prompt's adapter (`Engine.open`).
 
     With `pick_async` (a pick that leaves the ids on the device and hands back
     an object with `.dev` and `.wait()`) and an engine that has `step_decode`,
@@ -78,7 +80,8 @@ def generate(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int,
         limit = engine.cache.max_positions
         if len(p) + max_new_tokens > limit:
             raise ContextOverflow(len(p) + max_new_tokens, limit)
-    stops = set(int(s) for s in stop_token_ids)
+    stops = [set(int(s) for s in stop_token_ids) | set(int(s) for s in (stops_of[i] if stops_of else ()))
+             for i in range(len(prompts))]
     stats = stats if stats is not None else GenerationStats()
     outputs: List[List[int]] = [[] for _ in prompts]
     max_batch = max(1, min(max_batch, engine.cache.max_slots))
@@ -93,7 +96,7 @@ def generate(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int,
         seqs = {}
         try:
             for i in live:  # inside the try: a slot taken before an open() fails is given back
-                seqs[i] = engine.open()
+                seqs[i] = engine.open() if adapters is None or adapters[i] is None else engine.open(adapters[i])
             entries = [(seqs[i], list(prompts[i]), [len(prompts[i]) - 1]) for i in live]
             stats.prefill_tokens += sum(len(prompts[i]) for i in live)
             if ahead:
@@ -114,7 +117,7 @@ def generate(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int,
                     outputs[i].append(tok)
                     if on_token is not None:
                         on_token(i, tok)
-                    if len(outputs[i]) >= max_new_tokens or tok in stops:
+                    if len(outputs[i]) >= max_new_tokens or tok in stops[i]:
                         engine.close(seqs.pop(i))
                     else:
                         still.append(i)
@@ -170,7 +173,7 @@ def _decode_ahead(engine, entries, live, seqs, outputs, max_new_tokens, stops, p
             stats.decode_tokens += 0 if len(outputs[i]) == 1 else 1
             if on_token is not None:
                 on_token(i, tok)
-            if len(outputs[i]) >= max_new_tokens or tok in stops:
+            if len(outputs[i]) >= max_new_tokens or tok in stops[i]:
                 if i in goes_on:
                     ended.add(i)  # its row is in the step now running
                 else:

@@ -36,7 +36,7 @@ class DecodeGraph:
     WARMUP = 1  # eager decode steps per engine before the first capture
     MAX_CAPTURE_FAILURES = 3  # captures of one graph that something else may invalidate before it is an error
 
-    def __init__(self, engine, n_seqs: int, context_hint: int):
+    def __init__(self, engine, n_seqs: int, context_hint: int, adapted: bool = False):
         self.engine = engine
         self.n = n_seqs
         # kernels that size themselves by the longest context see this bucket's
@@ -44,13 +44,19 @@ class DecodeGraph:
         self.context_hint = context_hint
         _, total = layout(n_seqs, n_seqs, n_seqs)
         self.buffer = torch.zeros((total,), dtype=torch.int32, device=engine.device)
+        # each sequence's adapter, for a step in which some have one
+        self.adapter_ids = torch.zeros((n_seqs,), dtype=torch.int32, device=engine.device) if adapted else None
         self.graph = None
         self.logits = None
         self.calls = 0
         self.kernels = 0
         self.capture_failures = 0
 
-    def run(self, tokens, slots, starts, want, tokens_dev=None, borrow: bool = False) -> torch.Tensor:
+    def _forward(self, batch) -> torch.Tensor:
+        with self.engine.adapted(self.adapter_ids):
+            return self.engine.model.forward(batch, self.engine.cache)
+
+    def run(self, tokens, slots, starts, want, tokens_dev=None, borrow: bool = False, adapters=None) -> torch.Tensor:
         """`tokens_dev` (int32 [n] on the device), when given, takes the place of
         the host `tokens`: it is copied over the descriptor's token field on the
         stream, after the descriptor itself.  The logits are a copy of the
@@ -61,6 +67,8 @@ class DecodeGraph:
         if tokens_dev is not None:
             batch.tokens.copy_(tokens_dev)
         batch.context_hint = self.context_hint
+        if self.adapter_ids is not None:
+            eng.staging.copy(adapters, self.adapter_ids)
         if self.graph is None:
             # the first decode steps of a batch size run eagerly: they size every
             # lazily allocated buffer; later graphs of that size capture at once
@@ -74,7 +82,7 @@ class DecodeGraph:
             if eng._eager_decodes < self.WARMUP or first_of_size:
                 eng._eager_decodes += 1
                 eng._eager_sizes.add(self.n)
-                return eng.model.forward(batch, eng.cache)
+                return self._forward(batch)
             # capture: the eager call above has already sized every lazy buffer
             torch.cuda.synchronize()
             g = torch.cuda.CUDAGraph()
@@ -88,7 +96,7 @@ class DecodeGraph:
             gc.disable()
             try:
                 with torch.cuda.graph(g, pool=eng.graph_pool(), capture_error_mode="thread_local"):
-                    self.logits = eng.model.forward(batch, eng.cache)
+                    self.logits = self._forward(batch)
             except (CudaError, RuntimeError) as e:
                 # Something invalidated the capture all the same (a call that is not permitted
                 # while a stream captures): nothing of the step has run, so it runs eagerly now,
@@ -100,7 +108,7 @@ class DecodeGraph:
                 del g
                 torch.cuda.set_stream(stream)  # the capture's side stream may still be the current one
                 torch.cuda.synchronize()
-                return eng.model.forward(batch, eng.cache)
+                return self._forward(batch)
             finally:
                 if collecting:
                     gc.enable()

@@ -17,6 +17,7 @@ from .. import ops
 from ..cache.specs import KVSpec, StateSpec
 from ..config.spec import ModelSpec, RunEntry
 from ..config.spec import names_dict
+from ..errors import UnsupportedArchitecture
 from ..parts.block import PostNormBlock, ReadyRows
 from ..parts.registry import BLOCKS, EMBEDDING_TERMS, NORMS, TensorInfo
 
@@ -133,6 +134,33 @@ class CausalLM:
             term.bind(per_term.get(ti, {}))
         if self.spec.tie_word_embeddings:
             self.head = self.embedding  # the same storage, no copy
+
+    n_adapters = 0
+
+    def bind_adapters(self, adapters) -> None:
+        """`adapters`: what `weights.adapters.read_adapter` gave for each; they take the place of those bound before.
+        Nothing changes where one of them names a matrix that its part does not take adapters for."""
+        exp = expected_tensors(self.spec)
+        parts: Dict[Tuple[int, str], Dict[str, list]] = {}
+        for i, adapter in enumerate(adapters):
+            for name, pair in adapter.pairs.items():
+                where = exp[name][0]
+                if len(where) != 4:
+                    raise UnsupportedArchitecture(f"adapters for {name}: only the layers' projections have them")
+                _, li, part, role = where
+                if not getattr(getattr(self.layers[int(li)], part, None), "takes_adapters", False):
+                    raise UnsupportedArchitecture(f"adapters for {name}: its part takes none")
+                parts.setdefault((int(li), part), {}).setdefault(role, [None] * len(adapters))[i] = pair
+        scales = [a.scale for a in adapters]
+        made = []
+        for li, layer in enumerate(self.layers):
+            for name in ("mixer", "feed_forward"):
+                part = getattr(layer, name, None)
+                if getattr(part, "takes_adapters", False):
+                    made.append((part, part.adapter_banks(parts.get((li, name), {}), scales)))
+        for part, banks in made:
+            part.adapters = banks
+        self.n_adapters = len(adapters)
 
     # --- cache ------------------------------------------------------------
     def cache_entry_specs(self) -> Dict[int, Any]:

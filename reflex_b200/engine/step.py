@@ -17,6 +17,7 @@ from __future__ import annotations
 
 from typing import Dict, List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from ..cache.store import PAGE_TOKENS, Cache
@@ -50,7 +51,9 @@ class Engine:
         self.use_graphs = bool(use_graphs and model.dtype == torch.bfloat16 and model.capturable
                                and torch.device(self.device).type == "cuda")
         self.max_graphs = max(1, int(max_graphs))
-        self._graphs: Dict[Tuple[int, int], "object"] = {}  # insertion order = least recently used first
+        # by (sequences, context bucket, with adapters); insertion order = least recently used first
+        self._graphs: Dict[Tuple[int, int, bool], "object"] = {}
+        self._adapter_of: Dict[int, int] = {}  # sequences that go through one of the model's adapters
         self._graph_pool = None
         self._eager_decodes = 0  # eager decode steps run so far
         self._eager_sizes: set = set()  # batch sizes that have run eagerly once
@@ -62,13 +65,52 @@ class Engine:
         self.workspace = Workspace(self.device) if on_gpu else None
 
     # --- sequences ----------------------------------------------------------
-    def open(self) -> int:
-        """Start a sequence: takes a cache slot, returns its handle."""
-        return self.cache.take_slot()
+    def open(self, adapter: Optional[int] = None) -> int:
+        """Start a sequence: takes a cache slot, returns its handle.  `adapter`: the number of the model's adapter
+        (`load_adapters`) that all its tokens go through."""
+        if adapter is not None and not 0 <= adapter < self.model.n_adapters:
+            raise InvalidInput(f"adapter {adapter} is not among the model's {self.model.n_adapters}")
+        seq = self.cache.take_slot()
+        if adapter is not None:
+            self._adapter_of[seq] = int(adapter)
+        return seq
 
     def close(self, seq: int) -> None:
         """End a sequence: its slot and pages go back to the cache."""
         self.cache.give_slot(seq)
+        self._adapter_of.pop(seq, None)
+
+    def load_adapters(self, adapters) -> None:
+        """The model's adapters from now on, in place of earlier ones (`CausalLM.bind_adapters`); no sequence may be
+        open that uses one."""
+        if self._adapter_of:
+            raise InvalidInput("adapters cannot be exchanged while sequences that use them are open")
+        if torch.device(self.device).type == "cuda":
+            torch.cuda.synchronize(self.device)  # a step that reads the earlier ones may still run
+        self._graphs = {k: g for k, g in self._graphs.items() if not k[2]}  # captured steps point at the earlier ones
+        self.model.bind_adapters(adapters)
+
+    def _row_adapters(self, slots, counts=None):
+        """The adapter of every row of a step, -1 for none (NumPy int32); None where no sequence has one."""
+        if not any(s in self._adapter_of for s in slots):
+            return None
+        ids = np.fromiter((self._adapter_of.get(s, -1) for s in slots), dtype=np.int32, count=len(slots))
+        return ids if counts is None else np.repeat(ids, counts)
+
+    def adapted(self, ids: Optional[torch.Tensor]):
+        """The context in which a step's rows go through the adapters `ids` (int32 on the device; None: through none)."""
+        from .. import ops
+
+        return ops.use_adapters(None if ids is None else ops.adapter_rows(ids, self.model.n_adapters))
+
+    def _upload_adapters(self, ids) -> Optional[torch.Tensor]:
+        from ..ops.workspace import new
+
+        if ids is None:
+            return None
+        dev = new((len(ids),), torch.int32, self.device, keep=True)  # lives for the step
+        self.staging.copy(ids, dev)
+        return dev
 
     def length(self, seq: int) -> int:
         return self.cache.length(seq)
@@ -132,13 +174,15 @@ class Engine:
                     logits = self._decode_graphed(tokens, slots, starts, want, borrow=borrow)
                 else:
                     batch = make_batch(tokens, slots, starts, want, self.device, staging=self.staging)
-                    if head is not None:
-                        logits = head(batch)
-                    elif n_want:
-                        logits = self.model.forward(batch, cache)
-                    else:
-                        self.model.hidden_states(batch, cache, rows=batch.want_rows)  # nothing wanted: no rows
-                        logits = torch.empty((0, self.vocab_size), dtype=torch.float32, device=self.device)
+                    ids = self._upload_adapters(self._row_adapters(slots, [len(t) for t in tokens]))
+                    with self.adapted(ids):
+                        if head is not None:
+                            logits = head(batch)
+                        elif n_want:
+                            logits = self.model.forward(batch, cache)
+                        else:
+                            self.model.hidden_states(batch, cache, rows=batch.want_rows)  # nothing wanted: no rows
+                            logits = torch.empty((0, self.vocab_size), dtype=torch.float32, device=self.device)
             if self.workspace is not None:
                 self.workspace.settle()
         except Exception:
@@ -212,7 +256,8 @@ class Engine:
                 else:
                     batch = make_batch(tokens, slots, starts, want, self.device, staging=self.staging)
                     batch.tokens.copy_(tokens_dev)
-                    logits = self.model.forward(batch, cache)
+                    with self.adapted(self._upload_adapters(self._row_adapters(slots))):
+                        logits = self.model.forward(batch, cache)
             if self.workspace is not None:
                 self.workspace.settle()
         except Exception:
@@ -235,20 +280,21 @@ class Engine:
         # kernel's key splits, on how long the longest context is: one graph per
         # (batch size, context bucket)
         bucket = decode_context_bucket(max(starts) + 1, PAGE_TOKENS)
-        key = (n, bucket)
+        adapters = self._row_adapters(slots)
+        key = (n, bucket, adapters is not None)
         g = self._graphs.pop(key, None)
         if g is None:
-            g = DecodeGraph(self, n, bucket)
+            g = DecodeGraph(self, n, bucket, adapted=adapters is not None)
             while len(self._graphs) >= self.max_graphs:
                 self._graphs.pop(next(iter(self._graphs)))  # the least recently used
         self._graphs[key] = g  # most recently used last
-        return g.run(tokens, slots, starts, want, tokens_dev=tokens_dev, borrow=borrow)
+        return g.run(tokens, slots, starts, want, tokens_dev=tokens_dev, borrow=borrow, adapters=adapters)
 
     def launches_per_decode_step(self, n_seqs: int) -> int:
         """This library's kernels in one decode step of `n_seqs` sequences
         (counted when the step's graph was captured; 0 if it never ran)."""
         best = 0
-        for (n, _bucket), g in self._graphs.items():
+        for (n, _bucket, _adapted), g in self._graphs.items():
             if n == n_seqs:
                 best = max(best, g.kernels)
         return best

@@ -13,6 +13,7 @@ from typing import Optional
 import torch
 
 from ..errors import CudaError, InvalidInput
+import contextlib as _contextlib
 import os as _os
 
 from . import native, workspace
@@ -435,6 +436,24 @@ def adapter_rows(ids: torch.Tensor, n: int, tile: Optional[int] = None) -> Adapt
                                        tiles.data_ptr(), t, device_error_word(ids.device).data_ptr(), _stream())
     native.check(st, f"adapter_rows (R={R}, n={n})")
     return AdapterRows(order, first, tiles, tile)
+
+
+_ADAPTERS: Optional[AdapterRows] = None
+
+
+@_contextlib.contextmanager
+def use_adapters(rows: Optional[AdapterRows]):
+    """The rows' adapters that the parts of a model go by inside the block (None: no row has one)."""
+    global _ADAPTERS
+    prev, _ADAPTERS = _ADAPTERS, rows
+    try:
+        yield rows
+    finally:
+        _ADAPTERS = prev
+
+
+def active_adapters() -> Optional[AdapterRows]:
+    return _ADAPTERS
 
 
 class AdapterBank:

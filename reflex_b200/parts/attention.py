@@ -37,6 +37,7 @@ from .. import ops
 from ..cache.specs import KVSpec
 from ..config.spec import MixerSpec
 from ..errors import InvalidInput
+from .adapters import add, make_bank
 from .registry import NORMS, POSITIONS, TensorInfo, register_mixer
 
 
@@ -76,6 +77,7 @@ class GQAttention:
         self.o = None
         self.q_norm = None
         self.k_norm = None
+        self.adapters = (None, None)  # of the stacked projection, of the output projection
 
     @classmethod
     def tensor_specs(cls, spec: MixerSpec) -> Dict[str, TensorInfo]:
@@ -141,7 +143,23 @@ class GQAttention:
                 self.k_norm = tensors["k_norm"].to(device=self.device, dtype=torch.float32).contiguous()
 
     supports_fused_residual = True
-    accepts_normed_input = True  # its first product finishes a norm that the product before began
+
+    @property
+    def accepts_normed_input(self) -> bool:
+        """Its first product finishes a norm that the product before began (adapters take rows that are normed)."""
+        return self.adapters[0] is None or ops.active_adapters() is None
+
+    @property
+    def takes_adapters(self) -> bool:
+        return not (self.general or any_reader(self.spec))
+
+    def adapter_banks(self, pairs, scales):
+        s = self.spec
+        none = [None] * len(scales)
+        cols = (s.num_heads * s.head_dim, s.num_kv_heads * s.head_dim, s.num_kv_heads * s.head_dim)
+        return (make_bank([pairs.get(r, none) for r in ("q_proj", "k_proj", "v_proj")], cols, s.hidden_size, scales,
+                          self.dtype, self.device),
+                make_bank([pairs.get("o_proj", none)], (s.hidden_size,), cols[0], scales, self.dtype, self.device))
 
     @property
     def capturable(self) -> bool:
@@ -163,7 +181,8 @@ class GQAttention:
         norm = s.qk_norm
         if self.general:
             return self._forward_general(x, ctx, rotation)
-        if ops.qkv_fused_takes(x, s.head_dim, rotation, w):
+        qkv_adapters, o_adapters = self.adapters if ops.active_adapters() is not None else (None, None)
+        if qkv_adapters is None and ops.qkv_fused_takes(x, s.head_dim, rotation, w):
             # a few rows: norms, rotation and the cache write are the product's epilogue
             q = ops.qkv_fused(
                 x, w, self.q_norm, self.k_norm, norm.eps if norm else 0.0,
@@ -173,6 +192,7 @@ class GQAttention:
             ops.prof_mark("qkv_gemm")
         else:
             qkv = ops.linear(x, w, out_dtype=torch.float32 if x.shape[0] <= ops.GEMV_MAX_ROWS else None)
+            add(qkv, x, qkv_adapters)
             ops.prof_mark("qkv_gemm")
             q = ops.qkv_post(
                 qkv, self.q_norm, self.k_norm, norm.eps if norm else 0.0,
@@ -183,12 +203,12 @@ class GQAttention:
         attn = ops.attention(q, kv.k_pages, kv.v_pages, kv.page_table, kv.page_size, batch,
                              s.num_heads, s.num_kv_heads, s.head_dim, s.window, s.scale)
         ops.prof_mark("attn")
-        if residual is not None:
+        if residual is not None and o_adapters is None:
             fused = ops.linear_residual(attn, self.o, residual[0], residual[1])
             if fused is not None:
                 ops.prof_mark("o_proj")
                 return None if fused is ops.ADDED else fused  # None: nothing left to add
-        out = ops.linear(attn, self.o, out_dtype=torch.float32)
+        out = add(ops.linear(attn, self.o, out_dtype=torch.float32), attn, o_adapters)
         ops.prof_mark("o_proj")
         return out
 

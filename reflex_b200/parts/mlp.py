@@ -16,6 +16,7 @@ import torch
 
 from .. import ops
 from ..config.spec import FeedForwardSpec
+from .adapters import add, make_bank
 from .registry import TensorInfo, register_feed_forward
 
 
@@ -48,21 +49,37 @@ class SwiGLU:
         self.down = dev(tensors["down_proj"]).contiguous()
 
     supports_fused_residual = True
-    accepts_normed_input = True  # its first product finishes a norm that the product before began
+    takes_adapters = True
+    adapters = (None, None)  # of the woven projection, of the down projection
+
+    @property
+    def accepts_normed_input(self) -> bool:
+        """Its first product finishes a norm that the product before began (adapters take rows that are normed)."""
+        return self.adapters[0] is None or ops.active_adapters() is None
+
+    def adapter_banks(self, pairs, scales):
+        H, I, none = self.spec.hidden_size, self.spec.intermediate_size, [None] * len(scales)
+        return (make_bank([pairs.get(r, none) for r in ("gate_proj", "up_proj")], (I, I), H, scales, self.dtype,
+                          self.device, woven=True),
+                make_bank([pairs.get("down_proj", none)], (H,), I, scales, self.dtype, self.device))
 
     def forward(self, x, residual=None):
         """With `residual` = (hidden, next norm) the down projection may add itself
         to `hidden`; it then returns the rows for the product after that norm
         (`ops.NormedInput`) or None (added, the norm not begun).  Otherwise it
         returns the delta."""
-        act = ops.linear_swiglu(x, self.gate_up)
+        gate_up_adapters, down_adapters = self.adapters if ops.active_adapters() is not None else (None, None)
+        if gate_up_adapters is not None:
+            act = ops.swiglu(add(ops.linear(x, self.gate_up), x, gate_up_adapters), alternating=True)
+        else:
+            act = ops.linear_swiglu(x, self.gate_up)
         ops.prof_mark("ffn_gate_up")
-        if residual is not None:
+        if residual is not None and down_adapters is None:
             fused = ops.linear_residual(act, self.down, residual[0], residual[1])
             if fused is not None:
                 ops.prof_mark("ffn_down")
                 return None if fused is ops.ADDED else fused  # None: nothing left to add
-        out = ops.linear(act, self.down, out_dtype=torch.float32)
+        out = add(ops.linear(act, self.down, out_dtype=torch.float32), act, down_adapters)
         ops.prof_mark("ffn_down")
         return out
 
@@ -76,6 +93,7 @@ class GeGLU(SwiGLU):
 
     accepts_normed_input = False
     supports_fused_residual = False
+    takes_adapters = False
 
     def forward(self, x, residual=None):
         act = ops.linear_geglu(x, self.gate_up)

@@ -2,8 +2,9 @@
 (src/sampling.rs:41-66): `temperature <= 0` (the default) or NaN is greedy
 argmax with no random draw; a positive temperature samples from the softmax,
 after `top_k` (keep the k most probable) and then `top_p` (keep the shortest
-most-probable prefix whose probability reaches top_p); `seed` makes the draws
-reproducible; `stop_token_ids` end a generation (the stop token is kept).
+most-probable prefix whose probability reaches top_p) and `min_p` (keep what is
+at least min_p times as probable as the most probable token; this library's own);
+`seed` makes the draws reproducible; `stop_token_ids` end a generation (the stop token is kept).
 """
 
 from __future__ import annotations
@@ -23,6 +24,7 @@ class SamplingParams:
     top_p: Optional[float] = None
     seed: Optional[int] = None
     stop_token_ids: Tuple[int, ...] = ()
+    min_p: Optional[float] = None
 
     def is_greedy(self) -> bool:
         return math.isnan(self.temperature) or self.temperature <= 0.0
@@ -38,6 +40,8 @@ class SamplingParams:
             raise InvalidInput("sample: top_k must be at least 1")
         if self.top_p is not None and not (math.isfinite(self.top_p) and 0.0 <= self.top_p <= 1.0):
             raise InvalidInput(f"sample: top_p must be in [0, 1], got {self.top_p}")
+        if self.min_p is not None and not (math.isfinite(self.min_p) and 0.0 <= self.min_p <= 1.0):
+            raise InvalidInput(f"sample: min_p must be in [0, 1], got {self.min_p}")
 
 
 _MASK = (1 << 64) - 1

@@ -4,8 +4,9 @@ from __future__ import annotations
 
 import os
 import sys
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Union
 
+import numpy as np
 import torch
 
 from .. import ops
@@ -56,13 +57,22 @@ class PendingIds:
 
 class Sampler:
     """One generation call's chooser: greedy argmax, or temperature / top-k /
-    top-p with counter-based uniforms keyed by (seed, request, step)."""
+    top-p with counter-based uniforms keyed by (seed, request, step).  `params` may
+    be a list, one for each request of the call: every request then has its own
+    rules (and min-p), whatever shares its batch."""
 
-    def __init__(self, params: SamplingParams, device):
-        params.validate()
-        self.params = params
+    def __init__(self, params: Union[SamplingParams, Sequence[SamplingParams]], device):
+        every = [params] if isinstance(params, SamplingParams) else list(params)
+        for p in every:
+            p.validate()
+        self.params = every[0] if len(every) == 1 else None  # one for all requests
+        self.every = every
+        # rows with rules of their own go through `ops.sample_rows`
+        self.by_row = not isinstance(params, SamplingParams) or (params.min_p is not None and not params.is_greedy())
         self.device = device
-        self.seed = params.seed if params.seed is not None else fresh_seed()
+        fresh = fresh_seed()
+        self.seeds = [p.seed if p.seed is not None else fresh for p in every]
+        self.seed = self.seeds[0] if self.seeds else fresh
         self._const = {}
         self._scratch = None
         self._work = None
@@ -94,8 +104,8 @@ class Sampler:
                                 torch.zeros((1,), dtype=torch.int32, pin_memory=True))
         return ring["slots"][i]
 
-    def _upload_uniforms(self, values: List[float]) -> torch.Tensor:
-        """The step's uniform numbers on the device, through pinned buffers that
+    def _upload(self, values) -> torch.Tensor:
+        """The step's numbers (its uniform ones) on the device, through pinned buffers that
         take turns (a pick may still be in flight when the next is prepared)."""
         n = len(values)
         ring = self._uniforms.setdefault(n, {"next": 0, "slots": [None] * self.RING})
@@ -107,11 +117,29 @@ class Sampler:
                                 torch.cuda.Event())
         host, dev, copied = ring["slots"][i]
         copied.synchronize()  # the copy that last read this pinned buffer is done
-        for j, v in enumerate(values):
-            host[j] = v
+        host.copy_(torch.from_numpy(np.asarray(values, dtype=np.float32)))
         dev.copy_(host, non_blocking=True)
         copied.record()
         return dev
+
+    def _pick_rows(self, logits: torch.Tensor, requests: Sequence[int], steps: Sequence[int], out) -> None:
+        """Every row by its request's rules, which travel with the step's uniform numbers."""
+        n = len(requests)
+        mine = [0 if len(self.every) == 1 else r for r in requests]
+        rules = [self.every[i] for i in mine]
+
+        def numbers(name, off):
+            return [off if getattr(p, name) is None else getattr(p, name) for p in rules]
+
+        words = np.empty((5, n), dtype=np.float32)
+        words[0] = [uniform(self.seeds[i], r, s) for i, r, s in zip(mine, requests, steps)]
+        words[1] = [0.0 if p.is_greedy() else p.temperature for p in rules]
+        words[2], words[3] = numbers("top_p", 1.0), numbers("min_p", 0.0)
+        words[4].view(np.int32)[:] = [min(k, logits.shape[1]) for k in numbers("top_k", 0)]
+        u, t, p, m, k = self._upload(words.reshape(-1)).view(5, n)
+        has = [any(getattr(q, name) is not None for q in rules) for name in ("top_k", "top_p", "min_p")]
+        ops.sample_rows(logits, t, u, top_k=k.view(torch.int32) if has[0] else None, top_p=p if has[1] else None,
+                        min_p=m if has[2] else None, out=out)
 
     def pick_async(self, logits: torch.Tensor, requests: Sequence[int], steps: Sequence[int]) -> PendingIds:
         """As `pick`, without waiting: the ids stay on the device for the next
@@ -120,10 +148,12 @@ class Sampler:
         dev, scratch, host, event, err_host = self._slot(n)
         if TOP2_TRACE:
             trace_top2(logits, requests)
-        if self.params.is_greedy():
+        if self.by_row:
+            self._pick_rows(logits, requests, steps, dev)
+        elif self.params.is_greedy():
             ops.argmax(logits, out=dev, scratch=scratch)
         else:
-            u = self._upload_uniforms([uniform(self.seed, r, s) for r, s in zip(requests, steps)])
+            u = self._upload([uniform(self.seed, r, s) for r, s in zip(requests, steps)])
             t, k, tp = self._constants(n)
             if self._scratch is None or self._scratch.shape[0] < n or self._scratch.shape[1] != V:
                 self._scratch = torch.empty((n, V), dtype=torch.float32, device=self.device)
