@@ -31,7 +31,7 @@ namespace {
 
 using namespace rfx;
 
-constexpr int BINS = 2048, COARSE = 64, MAX_CLUSTER = 8, MAX_WARPS = 32, LIST = 256;
+constexpr int BINS = 2048, COARSE = 64, MAX_WARPS = 32, LIST = 256;
 constexpr int PER_OCTAVE = 32;               // bins an octave: e below 2^-64 of the maximum is nothing
 constexpr float FINE = PER_OCTAVE * (BINS / 2.0f);  // fine bins an octave: a bin and its roundings hold 2,048
 typedef unsigned long long u64;
@@ -111,16 +111,18 @@ struct Scale {
     }
 };
 
+// CLUSTER: the most CTAs a row may have.
+template <int CLUSTER>
 struct Shared {
     double table[PER_OCTAVE];  // 2^(-i / 32)
-    u64 coarse_m[COARSE], all_m[MAX_CLUSTER][COARSE];  // this CTA's, and every CTA's
-    u64 kept[MAX_CLUSTER], far[MAX_CLUSTER];
+    u64 coarse_m[COARSE], all_m[CLUSTER][COARSE];  // this CTA's, and every CTA's
+    u64 kept[CLUSTER], far[CLUSTER];
     u64 warp_m[MAX_WARPS];
     u64 mass_above, total;
-    int coarse_n[COARSE], all_n[MAX_CLUSTER][COARSE];
+    int coarse_n[COARSE], all_n[CLUSTER][COARSE];
     float list[LIST];
-    float top[MAX_CLUSTER];
-    int ties[MAX_CLUSTER], best[MAX_CLUSTER];
+    float top[CLUSTER];
+    int ties[CLUSTER], best[CLUSTER];
     int warp_i[MAX_WARPS];
     float warp_f[MAX_WARPS];
     int bin, above, in, who, listed;
@@ -183,7 +185,8 @@ __device__ __forceinline__ bool stops(const Rules& r, int count, u64 mass) {
 // The first bin, over the cluster's histograms, at which a rule stops the row; -1: none does.  Every CTA finds it
 // for itself, from 64 sums of 32 bins and then those 32.  `totals`: the bins hold the whole row but for the
 // mass that every CTA told apart (`far`), and the sum gives `want`.  The cluster meets once more before the histogram is used again.
-__device__ int choose(cg::cluster_group& cluster, Shared& sh, const Hist& hist, Rules& rules, bool totals) {
+template <int CLUSTER>
+__device__ int choose(cg::cluster_group& cluster, Shared<CLUSTER>& sh, const Hist& hist, Rules& rules, bool totals) {
     const int C = cluster.num_blocks(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     __syncthreads();
     for (int q = warp; q < COARSE; q += blockDim.x / 32) {
@@ -278,7 +281,8 @@ template <bool STAGED, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_rows_kernel(const Params p) {
     constexpr int WARPS = THREADS / 32;
     extern __shared__ __align__(16) uint8_t dynamic[];
-    __shared__ __align__(16) Shared sh;
+    // (rows with few CTAs beside them on an SM may have clusters of 16: two CTAs an SM have no room for that)
+    __shared__ __align__(16) Shared<THREADS == 1024 ? 16 : 8> sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = cluster.num_blocks(), c = cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -607,8 +611,11 @@ extern "C" int rfx_sample_rows(const float* logits, long long ld, int B, int V, 
                                void* stream) {
     if (B <= 0) return 0;
     if (V <= 0 || ld < V) return RFX_ERR_BAD_ARG;
+    // A cluster of 16 halves what its CTAs have to go over (a row of 151,936 with top-p: 23 -> 20 us), but a group of SMs
+    // holds one: eight rows took 16 us where clusters of eight take 11.
+    const int most = B <= 4 ? 16 : 8;
     int C = 1;
-    while (C < MAX_CLUSTER && (long long)C * 4096 < V && ((long long)B * C < 2 * sm_count() || (long long)C * 19200 < V)) C *= 2;
+    while (C < most && (long long)C * 4096 < V && ((long long)B * C < 2 * sm_count() || (long long)C * 19200 < V)) C *= 2;
     const int chunk = ((V + C - 1) / C + 3) / 4 * 4;
     const size_t hist = (size_t)BINS * 12, piece = (size_t)chunk * 4;
     const bool staged = hist + piece <= 200 * 1024;
@@ -623,6 +630,7 @@ extern "C" int rfx_sample_rows(const float* logits, long long ld, int B, int V, 
     static SmemLimit limits[4];
     auto go = [&](auto kernel, int threads, SmemLimit& limit) {
         cudaError_t e = limit.raise(kernel, smem);
+        if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) e = launch(kernel, dim3(B, 1, C), threads, smem, (cudaStream_t)stream, C, p);
         return (int)e;
     };
