@@ -198,6 +198,18 @@ def device_error_word(device) -> torch.Tensor:
     return _ERR[key]
 
 
+_ERR_PTR = {}
+
+
+def _error_word_of(t: torch.Tensor) -> int:
+    """The address of the error word of the device on which `t` lives."""
+    index = t.get_device()
+    p = _ERR_PTR.get(index)
+    if p is None:
+        p = _ERR_PTR[index] = device_error_word(t.device).data_ptr()
+    return p
+
+
 def check_device_errors(device="cuda:0") -> None:
     """Synchronises; raises if a kernel reported that a bounded wait ran out."""
     code = int(device_error_word(device).item())
@@ -413,29 +425,31 @@ class AdapterRows:
 
     def __init__(self, order: torch.Tensor, first: torch.Tensor, tiles: torch.Tensor, tile: int):
         self.order, self.first, self.tiles, self.tile = order, first, tiles, tile
-        self.n_rows, self.n, self.n_tiles = order.numel(), first.numel() - 2, tiles.shape[0]
-        self.order_ptr, self.tiles_ptr = order.data_ptr(), tiles.data_ptr()
+        self.n_rows, self.n, self.n_tiles = order.shape[0], first.shape[0] - 2, tiles.shape[0]
+        self.order_ptr, self.tiles_ptr = _chk(order, "order", torch.int32), _chk(tiles, "tiles", torch.int32)
 
 
 def adapter_rows(ids: torch.Tensor, n: int, tile: Optional[int] = None) -> AdapterRows:
     """Groups rows by `ids` (int32 [R], 0 .. n - 1, -1: no adapter) for the products of `adapter_add`: once a
     step, for all of them.  An id outside that range counts as none and is reported by `check_device_errors`."""
-    R = ids.numel()
+    if ids.dim() != 1 or ids.shape[0] == 0 or not 1 <= n <= 1024:
+        raise InvalidInput("adapter_rows: ids [rows], at least one, and 1 to 1024 adapters")
+    R = ids.shape[0]
     if tile is None:
         tile = 16 if R <= ADAPTER_STEP_ROWS else 128
-    if tile not in (16, 128):
+    if tile != 16 and tile != 128:
         raise InvalidInput(f"adapter_rows: tiles have 16 or 128 rows, not {tile}")
-    if ids.dim() != 1 or R == 0 or not 1 <= n <= 1024:
-        raise InvalidInput("adapter_rows: ids [rows], at least one, and 1 to 1024 adapters")
     _on_current(ids, "ids")
     t = min(R, n + 1) + R // tile
-    order = _new((R,), torch.int32, ids.device, keep=True)  # lives for the step
-    first = _new((n + 2,), torch.int32, ids.device, keep=True)
-    tiles = _new((t, 3), torch.int32, ids.device, keep=True)
-    st = native.lib().rfx_adapter_rows(_chk(ids, "ids", torch.int32), R, n, tile, order.data_ptr(), first.data_ptr(),
-                                       tiles.data_ptr(), t, device_error_word(ids.device).data_ptr(), _stream())
-    native.check(st, f"adapter_rows (R={R}, n={n})")
-    return AdapterRows(order, first, tiles, tile)
+    device = ids.device
+    order = _new((R,), torch.int32, device, keep=True)  # lives for the step
+    first = _new((n + 2,), torch.int32, device, keep=True)
+    tiles = _new((t, 3), torch.int32, device, keep=True)
+    rows = AdapterRows(order, first, tiles, tile)
+    st = native.lib().rfx_adapter_rows(_chk(ids, "ids", torch.int32), R, n, tile, rows.order_ptr, first.data_ptr(),
+                                       rows.tiles_ptr, t, _error_word_of(ids), _stream())
+    native.check(st, "adapter_rows")
+    return rows
 
 
 _ADAPTERS: Optional[AdapterRows] = None
@@ -511,7 +525,7 @@ class AdapterBank:
         form = native.lib().rfx_adapter_form
         self._form = {(tile, dt): form(self._ptr, tile, dt_code(dt))
                       for tile in (16, 128) for dt in (torch.float32, torch.bfloat16)}
-        self._err = device_error_word(a.device).data_ptr()
+        self._err = _error_word_of(a)
         self._index = a.get_device()
 
 

@@ -147,5 +147,5 @@ def new(shape, dtype, device, keep: bool = False, own: bool = False) -> torch.Te
     `own`: memory of its own that outlives the step (what a step returns)."""
     ws = _ACTIVE
     if own or ws is None or ws.device != torch.device(device):
-        return torch.empty(tuple(shape), dtype=dtype, device=device)
+        return torch.empty(shape, dtype=dtype, device=device)
     return ws.take(shape, dtype, keep=keep)
