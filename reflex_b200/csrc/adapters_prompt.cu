@@ -1,15 +1,19 @@
 // The adapters of prompts: tiles of up to 128 rows of one adapter, bfloat16, two launches.
 //
-//  * low: v = A x, 128 rows by all rank rows of all parts, on tcgen05 with 32-bit sums in tensor memory.  A's
-//    rows come by TMA, and so do the tile's where they follow one another (a prompt's); other tiles (where two prompts of one adapter meet, decoding rows by the hundred) are brought by
-//    four warps with 16-byte asynchronous copies straight into the operand's swizzled layout.  K goes in up to
-//    eight pieces while that fills the GPU, a tile's pieces are a cluster, and their sums meet in distributed
-//    shared memory, in order.  v goes to memory in two bfloat16 parts (16 bits: its error is 2^-9 of the result's
-//    rounding to bfloat16; three parts for a 32-bit result).  x is read once, and memory bounds it.
+//  * low: v = A x, 128 rows by all rank rows of all parts, on tcgen05 with 32-bit sums in tensor memory.  A's rows
+//    come by TMA, and so do the tile's where they follow one another (a prompt's); other tiles (where two prompts
+//    of one adapter meet, decoding rows by the hundred) are brought by four warps with 16-byte asynchronous copies
+//    straight into the operand's swizzled layout.  K goes in up to eight pieces while that fills the GPU, a tile's
+//    pieces are a cluster, and their sums meet in distributed shared memory, in order.  v goes to memory in two
+//    bfloat16 parts (16 bits: its error is 2^-9 of the result's rounding to bfloat16; three parts for a 32-bit
+//    result).  x is read once, A once a tile from the L2 cache.  8,192 rows by 4,096, three parts of rank 64: 30 to
+//    36 us where x alone would take 10; 2,047 rows by 12,288, rank 32: 25 us (x alone: 8).  What a block does once
+//    bounds it, the barriers, the pieces' meeting and the parts' stores, beside A's way out of the cache.
 //  * up: out = base + scale B v, 128 rows by up to 4,096 of one part's columns.  v comes by TMA as the operand that it
 //    is, B's columns follow by asynchronous copies, the products go to one of two accumulators in tensor
-//    memory, and four warps add them to base's rows, of which several groups of columns are always on their way.
-//    Base and out move in whole sectors, once: memory bounds it.
+//    memory, and sixteen warps add them to base's rows, of which several groups of columns are always on their way.
+//    Base and out move in whole sectors, once: memory bounds it (8,192 rows by 6,144 columns, 201 MB: 51 us, 3.9 TB/s,
+//    the first and the last columns of a block included, when it only reads or only writes).
 #include <cooperative_groups.h>
 
 #include "adapters.cuh"
@@ -28,10 +32,10 @@ using namespace sm100;
 constexpr int TILE = 128, BK = 64, LOW_THREADS = 384, MAX_STAGES = 8, MAX_W = 512, CHUNK = 256, MAX_PIECES = 8;
 constexpr int X_BYTES = TILE * BK * 2;
 
-// Blocks of 64 along K that each of `pieces` takes.
-__host__ __device__ inline int piece_blocks(int K, int pieces) {
-    const int blocks = (K + BK - 1) / BK;
-    return (blocks + pieces - 1) / pieces;
+// Stages, of `subs` blocks of 64 along K, that each of `pieces` takes.
+__host__ __device__ inline int piece_stages(int K, int subs, int pieces) {
+    const int all = (K + subs * BK - 1) / (subs * BK);
+    return (all + pieces - 1) / pieces;
 }
 
 // Shared memory by its own addresses: through generic ones a load takes several times as long, and the compiler orders
@@ -56,15 +60,15 @@ __device__ __forceinline__ void store_parts(__nv_bfloat16* dst, size_t apart, in
 
 __global__ void __launch_bounds__(LOW_THREADS)
 adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
-                      const __grid_constant__ CUtensorMap map_x, int box, int stages, int splits, uint32_t tmem_cols,
-                      int* __restrict__ err) {
+                      const __grid_constant__ CUtensorMap map_x, int box, int subs, int stages, int splits,
+                      uint32_t tmem_cols, int* __restrict__ err) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], done_bar;
     __shared__ uint32_t tmem_base;
     __shared__ int rows[TILE];
     uint8_t* stage0 = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int W = p.parts.n * p.rank, stage_bytes = X_BYTES + W * BK * 2;
+    const int W = p.parts.n * p.rank, stage_bytes = subs * (X_BYTES + W * BK * 2);
     pdl_wait();
     const Tile t = load_tile(p.tiles, blockIdx.x);
     if (t.adapter < 0 || t.adapter >= p.n) return;
@@ -72,8 +76,8 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
     // (a tile's pieces are a cluster; what returns here, returns as one)
     cg::cluster_group cluster = cg::this_cluster();
     const int pieces = cluster.num_blocks(), piece = cluster.block_rank();
-    const int per = piece_blocks(p.K, pieces), kb0 = piece * per;
-    const int nkb = min((p.K + BK - 1) / BK, kb0 + per) - kb0;  // (one at least)
+    const int step = subs * BK, per = piece_stages(p.K, subs, pieces), kb0 = piece * per;
+    const int nkb = min((p.K + step - 1) / step, kb0 + per) - kb0;  // (one at least)
     if (tid < TILE) rows[tid] = p.order[t.place + min(tid, t.count - 1)];
     const int row0 = p.order[t.place];
     const bool run = p.order[t.place + t.count - 1] - row0 == t.count - 1;  // (in order within a tile)
@@ -99,14 +103,15 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
     bool ok = true;
     if (warp < 4) {
         auto bring = [&](int s, int k) {  // A's rows of all parts, and the tile's where they follow one another
-            uint8_t* dst = stage0 + (size_t)s * stage_bytes;
-            mbar_expect_tx(&full_bar[s], (uint32_t)(W * BK * 2 + (run ? X_BYTES : 0)));
-            if (run) {
-                tma_load_2d(dst, &map_x, &full_bar[s], k, row0);
-                tma_load_2d(dst + X_BYTES / 2, &map_x, &full_bar[s], k, row0 + TILE / 2);
+            uint8_t *dst = stage0 + (size_t)s * stage_bytes, *a = dst + subs * X_BYTES;
+            mbar_expect_tx(&full_bar[s], (uint32_t)(subs * (W * BK * 2 + (run ? X_BYTES : 0))));
+            for (int b = 0; b < subs; ++b, k += BK, dst += X_BYTES) {
+                if (run) {
+                    tma_load_2d(dst, &map_x, &full_bar[s], k, row0);
+                    tma_load_2d(dst + X_BYTES / 2, &map_x, &full_bar[s], k, row0 + TILE / 2);
+                }
+                for (int w = 0; w < W; w += box, a += box * 128) tma_load_2d(a, &map_a, &full_bar[s], k, t.adapter * W + w);
             }
-            for (int w = 0; w < W; w += box)
-                tma_load_2d(dst + X_BYTES + w * 128, &map_a, &full_bar[s], k, t.adapter * W + w);
         };
         int s = 0, ph = 1;
         if (run) {
@@ -117,7 +122,7 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
                         ok = false;
                         break;
                     }
-                    bring(s, (kb0 + i) * BK);
+                    bring(s, (kb0 + i) * step);
                     if (++s == stages) s = 0, ph ^= 1;
                 }
             }
@@ -132,17 +137,18 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
                     break;
                 }
                 uint8_t* dst = stage0 + (size_t)s * stage_bytes;
-                const int k = (kb0 + i) * BK;
-                const bool in = k + u * 8 < p.K;
+                for (int b = 0; b < subs; ++b, dst += X_BYTES) {
+                    const int k = (kb0 + i) * step + b * BK + u * 8;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int r = r0 + 16 * j;
-                    const __nv_bfloat16* src = x + (size_t)rows[r] * p.ld_x + k + u * 8;
-                    attn::cp_async_16(dst + r * 128 + ((u ^ (r & 7)) << 4), in ? src : x, in);
+                    for (int j = 0; j < 8; ++j) {
+                        const int r = r0 + 16 * j;
+                        const __nv_bfloat16* src = x + (size_t)rows[r] * p.ld_x + k;
+                        attn::cp_async_16(dst + r * 128 + ((u ^ (r & 7)) << 4), k < p.K ? src : x, k < p.K);
+                    }
                 }
                 // this thread's arrival follows its copies
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_bar[s])) : "memory");
-                if (tid == 0) bring(s, k);
+                if (tid == 0) bring(s, (kb0 + i) * step);
                 if (++s == stages) s = 0, ph ^= 1;
             }
             attn::cp_async_wait<0>();
@@ -168,12 +174,14 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
                 // rows brought by threads were written by the generic proxy; the tensor cores read by the asynchronous one
                 if (!run) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 tc_fence_after_sync();
-                const uint64_t da = dx + X_BYTES / 16;
+                for (int b = 0; b < subs; ++b) {
+                    const uint64_t db = dx + b * (X_BYTES / 16), da = dx + subs * (X_BYTES / 16) + b * (W * 8);
 #pragma unroll
-                for (int k = 0; k < BK / 16; ++k) {
-                    umma_bf16(tmem, dx + 2 * k, da + 2 * k, idesc, more);
-                    if (W > 256) umma_bf16(tmem + 256, dx + 2 * k, da + 256 * 128 / 16 + 2 * k, idesc2, more);
-                    more = 1;
+                    for (int k = 0; k < BK / 16; ++k) {
+                        umma_bf16(tmem, db + 2 * k, da + 2 * k, idesc, more);
+                        if (W > 256) umma_bf16(tmem + 256, db + 2 * k, da + 256 * 8 + 2 * k, idesc2, more);
+                        more = 1;
+                    }
                 }
                 umma_commit(&empty_bar[s]);
                 dx += stage_step;
@@ -271,7 +279,7 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
 // both).  Warps 0 to 15 make the sums, 32 rows by every fourth 32 columns each; warp 16 issues the products, 17 and 18
 // bring B.  AHEAD groups of base a warp are on their way or in use, 128 KB where there is room: an SM that reads
 // and writes at its share of the memory's rate waits 3 to 4 us for a load, and with 64 KB on their way (two blocks
-// of four such warps) the kernel took 58 us where it now takes UP_US for 8,192 rows by 6,144 columns.  B's
+// of four such warps) the kernel took 58 us where it now takes 51 us for 8,192 rows by 6,144 columns.  B's
 // columns lie in the operand, and so in tensor memory, in an order that leaves a lane of the accumulator layout
 // with eight neighbours of a row: of a group of 32, column 4 n + j is number 8 j + n (woven: even j in the first
 // half of the turn's columns, odd j in the second, each half a product with its own part of v).
@@ -517,19 +525,23 @@ adapter_up_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_v, in
     }
 }
 
-// Pieces of K: the waves of blocks, an SM holding one, times the blocks of 64 that each takes and about eight for
-// its beginning and end, at their least; as few as give each a block.
-int pieces_of(int K, int max_tiles) {
-    const int blocks = (K + BK - 1) / BK, sms = sm_count();
+// Blocks of 64 along K a stage: two where at least two such stages have room, for a stage costs the thread that
+// issues its products about as much as their issue (2,047 rows by 12,288, rank 32: 28.5 us with one, 25 with two).
+int subs_of(int W) { return 2 * 2 * (X_BYTES + W * BK * 2) <= 200 * 1024 ? 2 : 1; }
+
+// Pieces of K: the waves of clusters times the stages that each block takes and what its beginning and end cost, at
+// their least; as few as give each a stage.
+int pieces_of(int K, int subs, int max_tiles) {
+    const int all = (K + subs * BK - 1) / (subs * BK), sms = sm_count();
     int best = 1;
     long long least = 0;
-    for (int n = 1; n <= MAX_PIECES && n <= (blocks + 3) / 4; ++n) {
+    for (int n = 1; n <= MAX_PIECES && n <= (all + 1) / 2; ++n) {
         const int at_once = n <= 2 ? sms / n : 8 * (18 / n);  // clusters: eight groups of 18 SMs or a few more
-        const long long cost = (long long)(max_tiles + at_once - 1) / at_once * ((blocks + n - 1) / n + 8);
+        const long long cost = (long long)(max_tiles + at_once - 1) / at_once * ((all + n - 1) / n * subs + 10);
         if (n == 1 || cost < least) best = n, least = cost;
     }
-    const int per = piece_blocks(K, best);
-    return (blocks + per - 1) / per;
+    const int per = piece_stages(K, subs, best);
+    return (all + per - 1) / per;
 }
 
 // Blocks of 64 along the rank that v takes in shared memory (16 KB each), all its bfloat16 parts together: beside
@@ -600,13 +612,13 @@ bool prompt_takes(const Args& p, int dt_out) {
 long long prompt_low_floats(int R, int W) { return ((long long)3 * R * W + 1) / 2; }  // three bfloat16 parts at most
 
 int prompt_form(const Args& p, int dt_out, int* err, cudaStream_t s) {
-    const int W = p.parts.n * p.rank, pieces = pieces_of(p.K, p.max_tiles);
+    const int W = p.parts.n * p.rank, subs = subs_of(W), pieces = pieces_of(p.K, subs, p.max_tiles);
     CUtensorMap map_a, map_x;
     const int box = W <= 256 ? W : 16;  // rows of A a copy brings (they come 53 cycles apart)
     if (!rfx::tma::make_map_rows64(&map_a, p.a, (long long)p.n * W, p.K, box) ||
         !rfx::tma::make_map_rows64(&map_x, p.x, p.R, p.K, TILE / 2, p.ld_x))
         return RFX_ERR_UNSUPPORTED;
-    const int stage = X_BYTES + W * BK * 2;
+    const int stage = subs * (X_BYTES + W * BK * 2);
     int stages = 200 * 1024 / stage;  // one block an SM: what is on its way hides the memory's latency
     if (stages < 2) stages = 2;
     if (stages > 6) stages = 6;
@@ -617,7 +629,7 @@ int prompt_form(const Args& p, int dt_out, int* err, cudaStream_t s) {
     cudaError_t e = limit.raise(adapter_low_tc_kernel, smem);
     if (e != cudaSuccess) return (int)e;
     const bool wide = dt_out == RFX_DT_F32;
-    e = launch(adapter_low_tc_kernel, dim3(p.max_tiles, 1, pieces), LOW_THREADS, smem, s, pieces, p, map_a, map_x, box, stages,
+    e = launch(adapter_low_tc_kernel, dim3(p.max_tiles, 1, pieces), LOW_THREADS, smem, s, pieces, p, map_a, map_x, box, subs, stages,
                wide ? 3 : 2, cols, err);
     if (e != cudaSuccess) return (int)e;
     if (wide) return p.parts.woven ? up<float, 3, true>(p, err, s) : up<float, 3, false>(p, err, s);
