@@ -424,6 +424,8 @@ class AdapterRows:
     `order`, rows; -1, 0, 0 behind the last."""
 
     def __init__(self, order: torch.Tensor, first: torch.Tensor, tiles: torch.Tensor, tile: int):
+        if tile != 16 and tile != 128:
+            raise InvalidInput(f"AdapterRows: tiles have 16 or 128 rows, not {tile}")
         self.order, self.first, self.tiles, self.tile = order, first, tiles, tile
         self.n_rows, self.n, self.n_tiles = order.shape[0], first.shape[0] - 2, tiles.shape[0]
         self.order_ptr, self.tiles_ptr = _chk(order, "order", torch.int32), _chk(tiles, "tiles", torch.int32)
@@ -549,12 +551,28 @@ def _rows_of(t: torch.Tensor, name: str) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices' rows share memory; columns of one wider matrix, side by side, do not."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    ld = a.stride(0) * a.element_size()
+    if a.shape[0] > 1 and b.shape[0] > 1 and ld == b.stride(0) * b.element_size():
+        apart = (b0 - a0) % ld  # b's rows begin so far behind a's
+        return not (apart >= a.shape[1] * a.element_size() and apart + b.shape[1] * b.element_size() <= ld)
+    return True
+
+
 def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, rows: AdapterRows,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """base + scale_a B_a (A_a x), row by row with the row's own adapter a (`rows`); a row without one is base's.
     `base` [R, N] float32, or bfloat16 beside a bfloat16 bank, is what the shared projection gave for `x` [R, K]
     (the bank's type); the sum is taken in 32-bit and rounded once.  `out` may be `base` itself: rows without an
-    adapter are then left alone.  Rows of base, x and out may lie apart."""
+    adapter are then left alone; else it overlaps neither base nor x.  Rows of base, x and out may lie apart.  Where
+    A_a x is not finite the row's sums may be NaN where the formula has an infinity."""
     ld_x, ld_base = _rows_of(x, "x"), _rows_of(base, "base")
     R, K = x.shape
     if K != bank.K or base.shape[0] != R or base.shape[1] != bank.N:
@@ -577,6 +595,9 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, rows: Ad
         ld_out = _rows_of(out, "out")
         if out.shape != base.shape or out.dtype != dtype:
             raise InvalidInput("adapter_add: out must be like base")
+        if out is not base and not (out.data_ptr() == base.data_ptr() and ld_out == ld_base) and (
+                _overlap(out, base) or _overlap(out, x)):
+            raise InvalidInput("adapter_add: out is base itself, or overlaps neither base nor x")
     xp = x.data_ptr()
     form = bank._form[rows.tile, dtype] if (xp | ld_x * 2) % 16 == 0 else 0
     lib = native.lib()
@@ -2530,8 +2551,11 @@ def sample_rows(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.
     off), `top_p` (>= 1: off), `min_p` (<= 0: off; tokens of at least min_p times the most probable one's
     probability) and its random number `uniform` in [0, 1).  Top-p's mass is that of the whole vocabulary; among
     equal logits the lower index is kept first; the draw walks the kept tokens in index order.  Logits of -inf or
-    NaN are never picked; a row with nothing else gives 0.  One launch, without working memory; exponentials and
-    sums are 64-bit, so a token is the one that exact arithmetic picks but for draws within 1e-12 of a border."""
+    NaN are never picked; a row with nothing else gives 0.  One launch, without working memory.  A token's mass is
+    good to 2e-9 of itself and sums do not depend on an order, so a token is the one that exact arithmetic picks but
+    for draws and cuts within about 2e-9 of the row's mass of a border."""
+    if temperature is None or uniform is None:
+        raise InvalidInput("sample_rows: every row needs a temperature and a random number")
     ld = _rows_of(logits, "logits")
     B, V = logits.shape
     if logits.dtype != torch.float32:

@@ -45,10 +45,12 @@ def read_adapter(folder: str, spec: ModelSpec) -> Adapter:
         raise IoError(f"{path}: cannot open: {e.strerror}") from e
     except ValueError as e:
         raise CheckpointError(f"{path} is not valid JSON: {e}") from None
+    if not isinstance(cfg, dict):
+        raise CheckpointError(f"{path}: a JSON object is needed")
     r, alpha = cfg.get("r"), cfg.get("lora_alpha")
     if isinstance(r, bool) or not isinstance(r, int) or r < 1:
         raise CheckpointError(f"{path}: r must be a positive integer, got {r!r}")
-    if isinstance(alpha, bool) or not isinstance(alpha, (int, float)) or not math.isfinite(alpha):
+    if isinstance(alpha, bool) or not isinstance(alpha, (int, float)) or not abs(alpha) < 2.0 ** 127:
         raise CheckpointError(f"{path}: lora_alpha must be a number, got {alpha!r}")
     for key, off in _OFF.items():
         if cfg.get(key, off) not in (off, None):

@@ -8,7 +8,7 @@ import torch
 
 import helpers
 from adapter_folders import adapter_folder
-from reflex_b200 import CheckpointError, InvalidInput, IoError, SamplingParams, UnsupportedArchitecture
+from reflex_b200 import CheckpointError, InvalidInput, IoError, SamplingParams, UnsupportedArchitecture, ops
 from reflex_b200.engine.generate import generate
 from reflex_b200.weights import write_safetensors
 from reflex_b200.weights.adapters import read_adapter
@@ -110,3 +110,34 @@ def test_min_p_is_checked():
     for bad in (-0.1, 1.1, float("nan")):
         with pytest.raises(InvalidInput, match="min_p"):
             SamplingParams(temperature=1.0, min_p=bad).validate()
+
+
+@pytest.mark.parametrize("text", ["[1, 2]", "7", '{"r": 4, "lora_alpha": 1%s}' % ("0" * 400)])
+def test_configurations_that_are_no_object_or_out_of_range(text):
+    folder, _ = adapter_folder(CFG, 4, 1)
+    with open(os.path.join(folder, "adapter_config.json"), "w") as f:
+        f.write(text)
+    with pytest.raises(CheckpointError):
+        read_adapter(folder, spec())
+
+
+def test_rows_in_tiles_that_no_kernel_has():
+    n = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(InvalidInput, match="16 or 128"):
+        ops.AdapterRows(n, n, n.view(2, 2), 32)
+
+
+def test_sampling_needs_a_temperature_and_a_number_a_row():
+    one = torch.ones(2)
+    for t, u in ((None, one), (one, None)):
+        with pytest.raises(InvalidInput, match="temperature"):
+            ops.sample_rows(torch.zeros(2, 5), t, u)
+
+
+def test_what_overlaps():
+    big = torch.zeros(6, 20)
+    for a, b, want in ((big[:, :8], big[:, 8:], False), (big[:, 8:], big[:, :8], False), (big[:, :9], big[:, 8:], True),
+                       (big[:3], big[3:], False), (big[:4, :8], big[2:, :8], True), (big[:4, :8], big[2:, 8:16], False),
+                       (big[1:, 12:], big[:5, :12], False), (big, big[2:3, 4:5], True), (big[:, :4], big.view(3, 40)[:, 4:8], True),
+                       (big, big.clone(), False), (big[:, :8], big.view(torch.int16).view(6, 40)[:, 16:], False)):
+        assert ops._overlap(a, b) is want

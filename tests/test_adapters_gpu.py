@@ -268,3 +268,20 @@ def test_refusals():
         ops.AdapterBank(a, b.float(), scale, QKV)
     with pytest.raises(bad):
         ops.AdapterBank(a, b, scale[:1], QKV)
+
+
+def test_a_result_that_overlaps_what_is_read():
+    base, x, a, b, scale, ids, bank = make(4, 160, QKV, 16, 2, torch.bfloat16, torch.bfloat16)
+    rows = ops.adapter_rows(ids, 2)
+    wide = torch.zeros(8, 160, dtype=torch.bfloat16, device=DEV)
+    wide[::2] = base
+    for out, was in ((x, base), (wide[1:5], wide[:4]), (wide[:4], wide[::2])):
+        with pytest.raises(ops.InvalidInput, match="overlaps"):
+            ops.adapter_add(was, x, bank, rows, out=out)
+    both = torch.zeros(4, 320, dtype=torch.bfloat16, device=DEV)  # side by side in the same rows is no overlap
+    both[:, :160] = base
+    ops.adapter_add(both[:, :160], x, bank, rows, out=both[:, 160:])
+    check(both[:, 160:].contiguous(), base, x, a, b, scale, ids, QKV, False)
+    view = base.view(4, 160)  # base itself by another tensor
+    before = base.clone()
+    check(ops.adapter_add(base, x, bank, rows, out=view), before, x, a, b, scale, ids, QKV, False)
