@@ -18,6 +18,11 @@
 // depend on the order in which threads add, and a draw near one of 150,000 borders between tokens lands on the
 // side that exact arithmetic gives (with plain 32-bit exponentials one row in ten thousand of a flat distribution
 // does not; 64-bit ones throughout are as good and cost as much as all the rest).
+//
+// The row is read once (64 rows of 151,936: 39 MB, 6 us at the memory's rate), but every logit costs a mass, a
+// histogram's atomics with a cut, and a place in a running sum: instructions bound it, and with few rows the
+// cluster's barriers.  Rows of 151,936: one with top-p 20 us, eight without a cut 11, 64 with all kinds of cuts 74;
+// 256 rows of 32,003 with all three 60.
 #include <cooperative_groups.h>
 #include <float.h>
 

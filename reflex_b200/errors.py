@@ -3,7 +3,8 @@
 The kinds and their numbers follow the reference's `ReflexErrorCode`
 (src/error.rs:72-90): values never change meaning and new kinds are only
 appended.  Kinds that belong to parts this library does not have (GGUF,
-tokenizer, LoRA, grammar) keep their numbers but are never raised; the
+tokenizer, grammar) keep their numbers but are never raised, nor is LoRA's (an
+adapter's folder has the faults of any checkpoint); the
 checkpoint-format kind (1) is used for safetensors / config.json faults, which
 is the role `Gguf` plays in the reference.
 """
