@@ -2,16 +2,18 @@
 //
 // A thread-block cluster takes a tile and both products.  Each of its eight CTAs multiplies the tile's rows
 // with A over an eighth of K on the tensor cores (m16n8k16: 16 rows, 8 rank rows), a warp every eighth 8 rank rows;
-// the partial sums meet in distributed shared memory, in rank order; then each CTA multiplies the low-rank rows
-// with its share of B's columns and adds the base.  Nothing but the result goes back to memory, and there is
-// one launch where two would have to follow one another.
+// the partial sums of a few rows go straight to all eight CTAs' shared memory (of many, each CTA fetches them there,
+// and the cluster meets once more: 0.5 us), and each adds them up in the same order; then it multiplies the low-rank
+// rows with its share of B's columns and adds the base.  Nothing but the result goes back to memory, and there is one
+// launch where two would have to follow one another.
 //
-// It is latency that counts, the chain tile -> row -> x and A -> cluster -> B, and then the adapters' bytes (an
-// adapter of rank 16 beside 4,096 x 6,144: 0.6 MB, which one row takes 6.5 us for; 64 rows over 32 adapters of
-// rank 64, 33 MB with base and out: 27 us).  So a warp
-// has 6 KB of A on their way, in a ring of shared memory of which every lane reads what it brought itself (no
-// barrier), k permuted alike on both sides so that a lane's elements lie side by side; B's columns are asked
-// for ahead, and a warp's first ones and their base are loaded before the cluster meets.
+// It is latency that counts, the chain tile -> row -> x and A -> cluster -> B, and then the adapters' bytes: one row
+// with an adapter of rank 16 beside 4,096 x 6,144 (0.6 MB) takes 5.8 us, 64 rows over 32 adapters of ranks to 64
+// (33 MB with base and out) 19 us, eight through 4,096 x 24,576 11 us.  So a warp's batches of A and then of B follow
+// one another through a ring of shared memory, 4 KB on their way, B's first while the cluster meets; every lane
+// reads what it brought itself (no barrier), k permuted alike on both sides so that its numbers lie side by side.
+// A deeper ring is slower (four batches: 20 us): at 64 rows the memory is busy as it is, and the adapters of small
+// rank then take more of it from those of large rank, which end last.
 //
 // The low-rank rows are kept in 32 bits and go into the second product as three bfloat16 parts (24 bits).
 // How K is cut depends on K alone, and a row's sums on nothing else in the tile, so a row has the same bits
@@ -29,19 +31,20 @@ using namespace rfx;
 using namespace adapters;
 
 constexpr int CLUSTER = 8, THREADS = 256, WARPS = THREADS / 32, TILE = 16;
-constexpr int RING = 3, BATCH = 4;          // a warp's batches of A under way, of 8 rank rows by 4 times 32 of K
-constexpr int GROUP = 32;                   // columns a warp makes at a time
-constexpr int AHEAD = 2;                    // steps of 16 along the rank whose B is loaded before the cluster meets
+constexpr int RING = 3;    // a warp's batches of A and B on their way or in use
+constexpr int BATCH = 4;   // of A: 8 rank rows by 4 times 32 of K; of B: a group of columns by 32 of the rank
+constexpr int GROUP = 32;  // columns a warp makes at a time
 
 // (in whole batches of 128)
 __host__ __device__ inline int k_slice(int K) { return ((K + CLUSTER - 1) / CLUSTER + 127) / 128 * 128; }
-// the warps' pieces of A, the rows of x, the partial rows, and the three parts' bfloat16s
-inline size_t step_smem(int W, int K) {
-    return (size_t)WARPS * RING * BATCH * 512 + (size_t)TILE * (k_slice(K) + 8) * 2 + (size_t)TILE * W * 4 +
-           (size_t)3 * TILE * (W + 8) * 2;
-}
-
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// elements from row to row: 64 bytes from where a row's banks begin, so that 16-byte reads by four lanes of two rows meet
+// different ones
+__host__ __device__ inline int ld_x_of(int K) { return k_slice(K) + 32; }
+__host__ __device__ inline int ld_v_of(int W) { return (W + 63) / 64 * 64 + 32; }
+// bytes of shared memory: the warps' rings; the rows of x and, when they have been read, v's three parts; partial rows
+__host__ __device__ inline int rows_bytes(int W, int K) { return max(TILE * ld_x_of(K) * 2, 3 * TILE * ld_v_of(W) * 2); }
+__host__ __device__ inline int sums_bytes(int W) { return max(TILE * W * 4, min(2 * TILE * W * 4, 24 * 1024)); }
+inline int step_smem(int W, int K) { return WARPS * RING * BATCH * 512 + rows_bytes(W, K) + sums_bytes(W); }
 
 __device__ __forceinline__ uint4 lds16(uint32_t at) {
     uint4 v;
@@ -55,16 +58,18 @@ __device__ __forceinline__ void load8(const TO* p, float (&v)[8]) {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
 template <typename TO>
 __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, int groups, int vec) {
     extern __shared__ __align__(16) uint8_t dynamic[];
-    __shared__ int rows[TILE];
     cg::cluster_group cluster = cg::this_cluster();
-    const int W = p.parts.n * p.rank, LDV = W + 8, slice = k_slice(p.K), LDX = slice + 8;
-    uint8_t* ring = dynamic;                                                              // [WARPS][RING][BATCH][lane]
+    const int W = p.parts.n * p.rank, LDV = ld_v_of(W), slice = k_slice(p.K), LDX = ld_x_of(p.K);
+    uint8_t* ring = dynamic;                                                                  // [WARPS][RING][BATCH][lane]
     __nv_bfloat16* xs = reinterpret_cast<__nv_bfloat16*>(ring + WARPS * RING * BATCH * 512);  // [TILE][LDX]
-    float* part_v = reinterpret_cast<float*>(xs + TILE * LDX);                            // [TILE][W]
-    __nv_bfloat16* vs = reinterpret_cast<__nv_bfloat16*>(part_v + TILE * W);              // [3][TILE][LDV]
+    __nv_bfloat16* vs = xs;                                                                   // [3][TILE][LDV]
+    float* sums = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(xs) + rows_bytes(W, p.K));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     pdl_prologue();
     const Tile tile = load_tile(p.tiles, blockIdx.y);
@@ -72,40 +77,23 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, 
     const bool none = tile.adapter >= p.n;
     if (none && p.out == p.base) return;
     const int count = min(tile.count, TILE), c = cluster.block_rank();
+    const int row_lo = p.order[tile.place + min(g, count - 1)], row_hi = p.order[tile.place + min(g + 8, count - 1)];
     const int rank = none ? 0 : p.rank_of(tile.adapter);
-    const int per = (rank + 7) / 8, steps = (rank + 15) / 16, tiles = per * p.parts.n;
-    // ---- a warp's first pieces of A: tiles of 8 rank rows n = warp, warp + 8, ..., 128 of K at a time; a lane brings,
-    // and reads, its own 16 bytes of each 32
-    const int k0 = c * slice, k1 = min(p.K, k0 + slice), blocks = k0 < k1 ? (k1 - k0 + 31) / 32 : 0;
-    const __nv_bfloat16* a = (const __nv_bfloat16*)p.a + (size_t)tile.adapter * W * p.lda;
-    const uint32_t my_ring = attn::smem_u32(ring) + warp * RING * BATCH * 512 + lane * 16;
-    int next_n = blocks ? warp : tiles, next_b = 0, next_slot = 0;
-    auto bring = [&]() {
-        if (next_n < tiles) {
-            const int s = next_n / per, row = s * p.rank + (next_n - s * per) * 8 + g;
-            const __nv_bfloat16* src = a + (size_t)row * p.lda + k0 + next_b * 32 + t * 8;
-#pragma unroll
-            for (int j = 0; j < BATCH; ++j) {
-                const int bytes = k0 + (next_b + j) * 32 + t * 8 < k1 ? 16 : 0;  // (zeros beyond)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(my_ring + (next_slot * BATCH + j) * 512),
-                             "l"(bytes ? src + j * 32 : a), "r"(bytes)
-                             : "memory");
-            }
-            if ((next_b += BATCH) >= blocks) next_b = 0, next_n += WARPS;
-            if (++next_slot == RING) next_slot = 0;
-        }
-        attn::cp_async_commit();
-    };
-    for (int i = 0; i < RING - 1; ++i) bring();
-    if (tid < TILE) rows[tid] = p.order[tile.place + min(tid, count - 1)];
-    __syncthreads();
+    const float scale = none ? 0.f : p.scale[tile.adapter];
+    const int per = (rank + 7) / 8, tiles = per * p.parts.n, b_batches = (per + 3) / 4;
+    if (!none) cluster_arrive();  // (the cluster's CTAs have begun: waited for before the first store to another)
     // ---- x's rows over this CTA's slice of K
+    const int k0 = c * slice, k1 = min(p.K, k0 + slice), blocks = k0 < k1 ? (k1 - k0 + 31) / 32 : 0;
     if (!none) {
         const __nv_bfloat16* x = (const __nv_bfloat16*)p.x;
         const int padded = (blocks + BATCH - 1) / BATCH * BATCH * 32;
-        for (int r = warp; r < count; r += WARPS)
-            for (int k = lane * 8; k < padded; k += 256)
-                attn::cp_async_16(xs + r * LDX + k, k0 + k < k1 ? x + (size_t)rows[r] * p.ld_x + k0 + k : x, k0 + k < k1);
+        const int rows[2] = {__shfl_sync(0xffffffffu, row_lo, warp * 4), __shfl_sync(0xffffffffu, row_hi, warp * 4)};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (warp + 8 * h < count)
+                for (int k = lane * 8; k < padded; k += 256)
+                    attn::cp_async_16(xs + (warp + 8 * h) * LDX + k, k0 + k < k1 ? x + (size_t)rows[h] * p.ld_x + k0 + k : x,
+                                      k0 + k < k1);
     }
     attn::cp_async_commit();
 
@@ -127,52 +115,74 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, 
         col = first + q * GROUP;
         end = p.parts.woven ? p.N : p.parts.end[part];
     };
-    auto load_b = [&](int col, int end, int s, int j) {  // step s of tile j: columns col + 4 n + j
-        const int at = min(col + 4 * g + j, end - 1);
-        return __ldg(reinterpret_cast<const uint2*>(b + (size_t)at * p.rank + s * 16 + t * 4));
+    // ---- a warp's batches of A, then of B: tiles of 8 rank rows n = warp, warp + 8, ..., 128 of K at a time, then its
+    // groups of columns, 32 of the rank at a time; a lane brings, and reads, its own 16 bytes of each 32 numbers
+    const __nv_bfloat16* a = (const __nv_bfloat16*)p.a + (size_t)tile.adapter * W * p.lda;
+    const uint32_t my_ring = attn::smem_u32(ring) + warp * RING * BATCH * 512 + lane * 16;
+    int next_n = blocks ? warp : tiles, next_b = 0, next_slot = 0, next_group = b_batches ? group : groups;
+    int next_part = 0, next_in = warp;  // tile next_n is number next_in of its part
+    auto settle = [&]() {
+        while (per && next_in >= per) next_in -= per, ++next_part;
     };
+    settle();
+    auto copy = [&](int j, const __nv_bfloat16* src, bool there) {  // (zeros if not)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(my_ring + (next_slot * BATCH + j) * 512),
+                     "l"(there ? src : a), "r"(there ? 16 : 0)
+                     : "memory");
+    };
+    auto bring = [&]() {
+        if (next_n < tiles) {
+            const int row = next_part * p.rank + next_in * 8 + g;
+            const __nv_bfloat16* src = a + (size_t)row * p.lda + k0 + next_b * 32 + t * 8;
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) copy(j, src + j * 32, k0 + (next_b + j) * 32 + t * 8 < k1);
+            if ((next_b += BATCH) >= blocks) {
+                next_b = 0, next_n += WARPS, next_in += WARPS;
+                settle();
+            }
+            if (++next_slot == RING) next_slot = 0;
+        } else if (next_group < groups) {
+            int col, end, part;
+            locate(next_group, col, end, part);
+            const int k = next_b * 32 + t * 8;
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j)  // tile j: columns col + 4 n + j
+                copy(j, b + (size_t)min(col + 4 * g + j, end - 1) * p.rank + k, k < per * 8);
+            if (++next_b == b_batches) next_b = 0, next_group += stride;
+            if (++next_slot == RING) next_slot = 0;
+        }
+        attn::cp_async_commit();
+    };
+    for (int i = 0; i < RING - 1; ++i) bring();
     const TO* base = (const TO*)p.base;
     TO* out = (TO*)p.out;
-    auto load_base = [&](int col, int end, int r, float (&v)[8]) {
+    auto load_base = [&](int col, int end, int r, int row, float (&v)[8]) {
         const int at = col + 8 * t;
         if (r < count) {
-            const TO* src = base + (size_t)rows[r] * p.ld_base + at;
+            const TO* src = base + (size_t)row * p.ld_base + at;
             if (vec && at + 8 <= end && (at & 7) == 0) load8(src, v);
             else
                 for (int i = 0; i < 8; ++i) v[i] = at + i < end ? ld(src, i) : 0.f;
         }
     };
-    uint2 ahead[AHEAD][4];
     float base_lo[8], base_hi[8];
     int col = 0, end = 0, part = 0;
-    const bool any = group < groups;
-    if (any) {
+    if (group < groups) {
         locate(group, col, end, part);
-#pragma unroll
-        for (int s = 0; s < AHEAD; ++s)
-            if (s < steps)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) ahead[s][j] = load_b(col, end, s, j);
-        load_base(col, end, g, base_lo);
-        load_base(col, end, g + 8, base_hi);
-        // this warp's columns of B and of base are asked for, and come from L2 when their turn has come
-        if (!none)
-            for (int q = group; q < groups; q += stride) {
-                int col_q, end_q, part_q;
-                locate(q, col_q, end_q, part_q);
-                const int n = min(GROUP, end_q - col_q) * p.rank;  // (one stretch of memory)
-                for (int i = lane * 64; i < n; i += 32 * 64) prefetch_l2(b + (size_t)col_q * p.rank + i);
-                if (q != group && lane < count) prefetch_l2(base + (size_t)rows[lane] * p.ld_base + col_q);
-            }
+        load_base(col, end, g, row_lo, base_lo);
+        load_base(col, end, g + 8, row_hi, base_hi);
     }
 
+    int slot = 0;
     if (!none) {
         // ---- the low-rank rows over this CTA's slice of K
-        for (int i = tid; i < 3 * TILE * LDV / 2; i += THREADS) reinterpret_cast<uint32_t*>(vs)[i] = 0u;
-        attn::cp_async_wait<0>();
+        attn::cp_async_wait<RING - 1>();
         __syncthreads();  // x is there
+        // (few rows: straight to where each CTA adds them up; else each CTA fetches them)
+        const int wide = tiles * 8;
+        const bool push = CLUSTER * count * wide * 4 <= sums_bytes(W);
+        cluster_wait();
         const uint32_t x_at = attn::smem_u32(xs) + (g * LDX + t * 8) * 2;
-        int slot = 0;
         for (int n = warp; n < tiles; n += WARPS) {
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
             for (int i = 0; i < blocks; i += BATCH) {
@@ -193,18 +203,29 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, 
                     attn::mma_bf16(acc, f1, w[j].z, w[j].w);
                 }
             }
-            store2(part_v + g * W + n * 8 + t * 2, acc[0], acc[1]);
-            store2(part_v + (g + 8) * W + n * 8 + t * 2, acc[2], acc[3]);
-        }
-        attn::cp_async_wait<0>();
-        cluster.sync();
-        // ---- the cluster's sums, in three parts of bfloat16
-        for (int i = tid; i < count * tiles * 8; i += THREADS) {
-            const int r = i / (tiles * 8), n = i - r * tiles * 8;
-            float v = 0.f;
+            if (push) {
 #pragma unroll
-            for (int q = 0; q < CLUSTER; ++q) v += cluster.map_shared_rank(part_v, q)[r * W + n];
-            const int s = n / (per * 8), at = r * LDV + s * p.rank + n - s * per * 8;
+                for (int q = 0; q < CLUSTER; ++q) {
+                    float* to = cluster.map_shared_rank(sums, q) + c * count * wide + n * 8 + t * 2;
+                    if (g < count) store2(to + g * wide, acc[0], acc[1]);
+                    if (g + 8 < count) store2(to + (g + 8) * wide, acc[2], acc[3]);
+                }
+            } else {
+                store2(sums + g * wide + n * 8 + t * 2, acc[0], acc[1]);
+                store2(sums + (g + 8) * wide + n * 8 + t * 2, acc[2], acc[3]);
+            }
+        }
+        cluster_arrive();
+        cluster_wait();
+        // ---- the cluster's sums, in three parts of bfloat16
+        for (int i = tid; i < count * wide; i += THREADS) {
+            const int r = i / wide, n = i - r * wide;
+            float d[CLUSTER], v = 0.f;
+#pragma unroll
+            for (int q = 0; q < CLUSTER; ++q) d[q] = push ? sums[q * count * wide + i] : cluster.map_shared_rank(sums, q)[i];
+#pragma unroll
+            for (int q = 0; q < CLUSTER; ++q) v += d[q];
+            const int at = r * LDV + n;
             const __nv_bfloat16 hi = __float2bfloat16_rn(v);
             const float rest = v - __bfloat162float(hi);
             const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
@@ -212,50 +233,59 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, 
             vs[TILE * LDV + at] = mid;
             vs[2 * TILE * LDV + at] = __float2bfloat16_rn(rest - __bfloat162float(mid));
         }
-        cluster.sync();  // no CTA leaves while another reads its sums
+        if (push) __syncthreads();
+        else {  // no CTA leaves while another reads its sums
+            cluster_arrive();
+            cluster_wait();
+        }
     }
 
     // ---- the columns
-    const float scale = none ? 0.f : p.scale[tile.adapter];
-    for (bool first = true; group < groups; group += stride, first = false) {
-        if (!first) {
-            locate(group, col, end, part);
-            load_base(col, end, g, base_lo);
-            load_base(col, end, g + 8, base_hi);
+    const uint32_t v_at = attn::smem_u32(vs) + (g * LDV + t * 8) * 2;
+    for (; group < groups; group += stride) {
+        // the next group's base is on its way meanwhile
+        int next_col = 0, next_end = 0, next_part = 0;
+        float next_lo[8], next_hi[8];
+        if (group + stride < groups) {
+            locate(group + stride, next_col, next_end, next_part);
+            load_base(next_col, next_end, g, row_lo, next_lo);
+            load_base(next_col, next_end, g + 8, row_hi, next_hi);
         }
         float acc[4][4] = {};
-        for (int s0 = 0; s0 < steps; s0 += AHEAD) {
-            if (!first || s0)
+        for (int i = 0; i < b_batches; ++i) {
+            bring();
+            attn::cp_async_wait<RING - 1>();
+            uint4 w[BATCH];
 #pragma unroll
-                for (int s = 0; s < AHEAD; ++s)
-                    if (s0 + s < steps)
+            for (int j = 0; j < BATCH; ++j) w[j] = lds16(my_ring + (slot * BATCH + j) * 512);
+            if (++slot == RING) slot = 0;
+            const bool there = i * 32 + t * 8 < per * 8;  // (what lies beyond is no number of this part)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) ahead[s][j] = load_b(col, end, s0 + s, j);
-#pragma unroll
-            for (int s = 0; s < AHEAD; ++s)
-                if (s0 + s < steps)
-#pragma unroll
-                    for (int q = 0; q < 3; ++q) {
-                        const __nv_bfloat16* v = vs + q * TILE * LDV + (s0 + s) * 16 + t * 4;
-                        auto frag = [&](int sp, uint32_t (&f)[4]) {
-                            const uint2 lo = *reinterpret_cast<const uint2*>(v + g * LDV + sp * p.rank);
-                            const uint2 hi = *reinterpret_cast<const uint2*>(v + (g + 8) * LDV + sp * p.rank);
-                            f[0] = lo.x, f[1] = hi.x, f[2] = lo.y, f[3] = hi.y;
-                        };
-                        uint32_t f[4], odd[4];
-                        frag(part, f);
-                        if (p.parts.woven) frag(1, odd);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if ((j & 1) && p.parts.woven) attn::mma_bf16(acc[j], odd, ahead[s][j].x, ahead[s][j].y);
-                            else attn::mma_bf16(acc[j], f, ahead[s][j].x, ahead[s][j].y);
-                        }
-                    }
+            for (int q = 0; q < 3; ++q) {
+                auto frag = [&](int sp, uint4& lo, uint4& hi) {
+                    const uint32_t at = v_at + (q * TILE * LDV + sp * per * 8 + i * 32) * 2;
+                    lo = hi = make_uint4(0, 0, 0, 0);
+                    if (there && g < count) lo = lds16(at);
+                    if (there && g + 8 < count) hi = lds16(at + 8 * LDV * 2);
+                };
+                auto multiply = [&](int j, const uint4& lo, const uint4& hi) {
+                    const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
+                    attn::mma_bf16(acc[j], f0, w[j].x, w[j].y);
+                    attn::mma_bf16(acc[j], f1, w[j].z, w[j].w);
+                };
+                uint4 lo, hi;
+                frag(part, lo, hi);
+                multiply(0, lo, hi);
+                multiply(2, lo, hi);
+                if (p.parts.woven) frag(1, lo, hi);
+                multiply(1, lo, hi);
+                multiply(3, lo, hi);
+            }
         }
-        auto store = [&](int r, const float (&y)[8], int h) {
+        auto store = [&](int r, int row, const float (&y)[8], int h) {
             const int at = col + 8 * t;
             if (r >= count) return;
-            TO* dst = out + (size_t)rows[r] * p.ld_out + at;
+            TO* dst = out + (size_t)row * p.ld_out + at;
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = none ? y[i] : fmaf(scale, acc[i & 3][h + (i >> 2)], y[i]);
@@ -268,8 +298,11 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, 
                     if (at + i < end) st(dst, i, v[i]);
             }
         };
-        store(g, base_lo, 0);
-        store(g + 8, base_hi, 2);
+        store(g, row_lo, base_lo, 0);
+        store(g + 8, row_hi, base_hi, 2);
+        col = next_col, end = next_end, part = next_part;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) base_lo[i] = next_lo[i], base_hi[i] = next_hi[i];
     }
 }
 
@@ -286,10 +319,10 @@ int go(const Args& p, cudaStream_t s) {
     if (share < 1) share = 1;
     const int most = (groups + CLUSTER * WARPS - 1) / (CLUSTER * WARPS);
     if (share > most) share = most;
-    const size_t smem = step_smem(W, p.K);
     // rows of base and out by 16 bytes
     const size_t align = (size_t)p.base | (size_t)p.out | (size_t)(p.ld_base * sizeof(TO)) | (size_t)(p.ld_out * sizeof(TO));
     const int vec = (align & 15) == 0;
+    const size_t smem = step_smem(W, p.K);
     static SmemLimit limit;
     cudaError_t e = limit.raise(adapter_step_kernel<TO>, smem);
     if (e == cudaSuccess)
