@@ -18,6 +18,7 @@ import os as _os
 
 from . import native, workspace
 from .workspace import new as _new
+from .workspace import new_like as _new_like
 
 F32, BF16 = 0, 1
 
@@ -426,9 +427,33 @@ class AdapterRows:
     def __init__(self, order: torch.Tensor, first: torch.Tensor, tiles: torch.Tensor, tile: int):
         if tile != 16 and tile != 128:
             raise InvalidInput(f"AdapterRows: tiles have 16 or 128 rows, not {tile}")
-        self.order, self.first, self.tiles, self.tile = order, first, tiles, tile
+        if order.dim() != 1 or first.dim() != 1 or first.shape[0] < 3 or tiles.dim() != 2 or tiles.shape[1] != 3:
+            raise InvalidInput("AdapterRows: order [rows], first [adapters + 2] and tiles [tiles, 3] are needed")
+        self._memory, self._parts, self.tile, self.index = None, (order, first, tiles), tile, order.get_device()
         self.n_rows, self.n, self.n_tiles = order.shape[0], first.shape[0] - 2, tiles.shape[0]
         self.order_ptr, self.tiles_ptr = _chk(order, "order", torch.int32), _chk(tiles, "tiles", torch.int32)
+
+    @classmethod
+    def _new(cls, device, index: int, n_rows: int, n: int, tile: int) -> "AdapterRows":
+        """In one piece of memory; the three parts are made when they are asked for."""
+        rows = cls.__new__(cls)
+        rows.n_rows, rows.n, rows.tile, rows.index = n_rows, n, tile, index
+        rows.n_tiles = min(n_rows, n + 1) + n_rows // tile
+        rows._memory = _new((n_rows + n + 2 + 3 * rows.n_tiles,), torch.int32, device, keep=True)  # lives for the step
+        rows._parts = None
+        rows.order_ptr = rows._memory.data_ptr()
+        rows.tiles_ptr = rows.order_ptr + 4 * (n_rows + n + 2)
+        return rows
+
+    def _part(self, i: int) -> torch.Tensor:
+        if self._parts is None:
+            order, first, tiles = self._memory.split_with_sizes((self.n_rows, self.n + 2, 3 * self.n_tiles))
+            self._parts = order, first, tiles.view(-1, 3)
+        return self._parts[i]
+
+    order = property(lambda self: self._part(0))
+    first = property(lambda self: self._part(1))
+    tiles = property(lambda self: self._part(2))
 
 
 def adapter_rows(ids: torch.Tensor, n: int, tile: Optional[int] = None) -> AdapterRows:
@@ -442,14 +467,10 @@ def adapter_rows(ids: torch.Tensor, n: int, tile: Optional[int] = None) -> Adapt
     if tile != 16 and tile != 128:
         raise InvalidInput(f"adapter_rows: tiles have 16 or 128 rows, not {tile}")
     _on_current(ids, "ids")
-    t = min(R, n + 1) + R // tile
-    device = ids.device
-    order = _new((R,), torch.int32, device, keep=True)  # lives for the step
-    first = _new((n + 2,), torch.int32, device, keep=True)
-    tiles = _new((t, 3), torch.int32, device, keep=True)
-    rows = AdapterRows(order, first, tiles, tile)
-    st = native.lib().rfx_adapter_rows(_chk(ids, "ids", torch.int32), R, n, tile, rows.order_ptr, first.data_ptr(),
-                                       rows.tiles_ptr, t, _error_word_of(ids), _stream())
+    ids_ptr = _chk(ids, "ids", torch.int32)
+    rows = AdapterRows._new(ids.device, ids.get_device(), R, n, tile)
+    st = native.lib().rfx_adapter_rows(ids_ptr, R, n, tile, rows.order_ptr, rows.order_ptr + 4 * R, rows.tiles_ptr,
+                                       rows.n_tiles, _error_word_of(ids), _stream())
     native.check(st, "adapter_rows")
     return rows
 
@@ -583,13 +604,13 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, rows: Ad
     if rows.n_rows != R or rows.n != bank.n:
         raise InvalidInput(f"adapter_add: the rows were grouped for {rows.n_rows} rows and {rows.n} adapters, "
                            f"not {R} and {bank.n}")
-    if bank._index != x.get_device() or rows.order.get_device() != bank._index:
+    if bank._index != x.get_device() or rows.index != bank._index:
         raise InvalidInput("adapter_add: x, base, the adapters and the rows live on one device")
     dtype = base.dtype
     if dtype != torch.float32 and dtype != bank.dtype:
         raise InvalidInput(f"adapter_add: base is {dtype} beside adapters in {bank.dtype}")
     if out is None:
-        out = _new((R, bank.N), dtype, base.device)
+        out = _new_like(base) if ld_base == bank.N else _new((R, bank.N), dtype, base.device)
         ld_out = bank.N
     else:
         ld_out = _rows_of(out, "out")

@@ -149,3 +149,8 @@ def new(shape, dtype, device, keep: bool = False, own: bool = False) -> torch.Te
     if own or ws is None or ws.device != torch.device(device):
         return torch.empty(shape, dtype=dtype, device=device)
     return ws.take(shape, dtype, keep=keep)
+
+
+def new_like(t: torch.Tensor) -> torch.Tensor:
+    """`new` for a result of a contiguous tensor's shape and type, beside it (outside a step a little cheaper)."""
+    return torch.empty_like(t) if _ACTIVE is None else new(t.shape, t.dtype, t.device)

@@ -125,6 +125,9 @@ def test_rows_in_tiles_that_no_kernel_has():
     n = torch.zeros(4, dtype=torch.int32)
     with pytest.raises(InvalidInput, match="16 or 128"):
         ops.AdapterRows(n, n, n.view(2, 2), 32)
+    for order, first, tiles in ((n, n, n.view(2, 2)), (n.view(2, 2), n, n[:3].view(1, 3)), (n, n[:2], n[:3].view(1, 3))):
+        with pytest.raises(InvalidInput, match="order"):
+            ops.AdapterRows(order, first, tiles, 16)
 
 
 def test_sampling_needs_a_temperature_and_a_number_a_row():
