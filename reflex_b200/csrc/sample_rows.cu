@@ -634,8 +634,7 @@ extern "C" int rfx_sample_rows(const float* logits, long long ld, int B, int V, 
     const size_t smem = hist + (staged ? piece : 0);
     static SmemLimit limits[4];
     auto go = [&](auto kernel, int threads, SmemLimit& limit) {
-        cudaError_t e = limit.raise(kernel, smem);
-        if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        cudaError_t e = limit.raise(kernel, smem, C > 8);
         if (e == cudaSuccess) e = launch(kernel, dim3(B, 1, C), threads, smem, (cudaStream_t)stream, C, p);
         return (int)e;
     };
