@@ -9,9 +9,9 @@
 //
 // A thread-block cluster takes a row: its CTAs hold a piece of it each in shared memory, so the logits are
 // read once, and exchange maxima, sums and histograms through distributed shared memory; one launch does
-// everything.  For top-k and top-p the cut is found in a histogram of 2,048 bins of 1/32 octave of e; the few
-// entries of the chosen bin go to every CTA, which finds the cut among them.  Where they are many, 2,048 bins
-// inside the bin follow, and, if several share one of those too (equal logits, a temperature that makes all
+// everything.  For top-k and top-p the cut is found in a histogram of 2,048 bins of 1/32 octave of e; the entries
+// of the chosen bin, up to 512 or 1,024, go to every CTA, and the cut is found among them.  Where they are more, 2,048
+// bins inside the bin follow, and, if several share one of those too (equal logits, a temperature that makes all
 // alike), their bit patterns are narrowed 2,048 bins at a time until one value is left.
 //
 // A mass is good to 2e-9 of itself (about 24 instructions: see `Scale`) and sums are 64-bit fixed point: they do not
@@ -21,8 +21,8 @@
 //
 // The row is read once (64 rows of 151,936: 39 MB, 6 us at the memory's rate), but every logit costs a mass, a
 // histogram's atomics with a cut, and a place in a running sum: instructions bound it, and with few rows the
-// cluster's barriers.  Rows of 151,936: one with top-p 20 us, eight without a cut 11, 64 with all kinds of cuts 74;
-// 256 rows of 32,003 with all three 60.
+// cluster's barriers.  Rows of 151,936: one with top-p 15 to 22 us, eight without a cut 11, 64 with all kinds of cuts 57;
+// 256 rows of 32,003 with all three 54.
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -36,7 +36,7 @@ namespace {
 
 using namespace rfx;
 
-constexpr int BINS = 2048, COARSE = 64, MAX_WARPS = 32, LIST = 256;
+constexpr int BINS = 2048, COARSE = 64, MAX_WARPS = 32;
 constexpr int PER_OCTAVE = 32;               // bins an octave: e below 2^-64 of the maximum is nothing
 constexpr float FINE = PER_OCTAVE * (BINS / 2.0f);  // fine bins an octave: a bin and its roundings hold 2,048
 typedef unsigned long long u64;
@@ -116,9 +116,11 @@ struct Scale {
     }
 };
 
-// CLUSTER: the most CTAs a row may have.
-template <int CLUSTER>
+// CLUSTER: the most CTAs a row may have; LIST: the most entries of a bin among which the cut is looked for one by one.
+template <int CLUSTER, int LIST_>
 struct Shared {
+    static constexpr int LIST = LIST_;
+    u64 list_m[LIST];
     double table[PER_OCTAVE];  // 2^(-i / 32)
     u64 coarse_m[COARSE], all_m[CLUSTER][COARSE];  // this CTA's, and every CTA's
     u64 kept[CLUSTER], far[CLUSTER];
@@ -190,8 +192,8 @@ __device__ __forceinline__ bool stops(const Rules& r, int count, u64 mass) {
 // The first bin, over the cluster's histograms, at which a rule stops the row; -1: none does.  Every CTA finds it
 // for itself, from 64 sums of 32 bins and then those 32.  `totals`: the bins hold the whole row but for the
 // mass that every CTA told apart (`far`), and the sum gives `want`.  The cluster meets once more before the histogram is used again.
-template <int CLUSTER>
-__device__ int choose(cg::cluster_group& cluster, Shared<CLUSTER>& sh, const Hist& hist, Rules& rules, bool totals) {
+template <typename Sh>
+__device__ int choose(cg::cluster_group& cluster, Sh& sh, const Hist& hist, Rules& rules, bool totals) {
     const int C = cluster.num_blocks(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     __syncthreads();
     for (int q = warp; q < COARSE; q += blockDim.x / 32) {
@@ -287,7 +289,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_rows_kernel(co
     constexpr int WARPS = THREADS / 32;
     extern __shared__ __align__(16) uint8_t dynamic[];
     // (rows with few CTAs beside them on an SM may have clusters of 16: two CTAs an SM have no room for that)
-    __shared__ __align__(16) Shared<THREADS == 1024 ? 16 : 8> sh;
+    using Sh = std::conditional_t<THREADS == 1024, Shared<16, 1024>, Shared<8, 512>>;
+    __shared__ __align__(16) Sh sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = cluster.num_blocks(), c = cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -425,9 +428,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_rows_kernel(co
             auto in_bin = [&](float l) {
                 return l >= from && !(l < bin_from || l > bin_to) && min(scale.template at<WIDE>(l).bin, BINS - 1) == bin;
             };
-            if (bin >= 0 && rules.in > 1 && rules.in <= LIST) {
+            if (bin >= 0 && rules.in > 1 && rules.in <= Sh::LIST) {
                 // the bin's entries to every CTA, in any order, and the cut among them: the largest value at which a
-                // rule stops the row
+                // rule stops the row, eight lanes an entry
 #pragma unroll 4
                 for (int i = tid; i < n; i += THREADS) {
                     const float l = at(i);
@@ -437,23 +440,44 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_rows_kernel(co
                     }
                 }
                 cluster.sync();
-                if (tid < rules.in) {
-                    const float l = sh.list[tid];
-                    int above = rules.above, equal = 0;
-                    u64 mass_above = rules.mass_above;
-                    for (int i = 0; i < rules.in; ++i) {
+                for (int i = tid; i < rules.in; i += THREADS)
+                    sh.list_m[i] = rules.p_on ? scale.mass(scale.template at<WIDE>(sh.list[i]), sh.table) : 0ull;
+                __syncthreads();
+                // (more than 64 comparisons a thread: each CTA takes its share and tells the others, one more meeting of
+                // 1.7 us; 64 rows of 151,936 with all kinds of cuts took 67 us on average where it now takes 57)
+                const bool shared = C > 1 && rules.in * rules.in > 64 * THREADS;
+                const int step = shared ? C : 1, mine = shared ? c : 0;
+                for (int e0 = 0; e0 < rules.in; e0 += step * (THREADS / 8)) {
+                    const int e = e0 + mine + step * (tid >> 3);
+                    const float l = e < rules.in ? sh.list[e] : 0.f;
+                    int above = 0, equal = 0;
+                    u64 mass_above = 0;
+#pragma unroll 4
+                    for (int i = tid & 7; i < rules.in; i += 8) {
                         const float o = sh.list[i];
-                        if (o > l) {
-                            ++above;
-                            if (rules.p_on) mass_above += scale.mass(scale.template at<WIDE>(o), sh.table);
-                        }
+                        const u64 m = sh.list_m[i];
+                        above += o > l;
+                        mass_above += o > l ? m : 0ull;
                         equal += o == l;
                     }
-                    const u64 each = rules.p_on ? scale.mass(scale.template at<WIDE>(l), sh.table) : 0ull;
-                    if (!stops(rules, above, mass_above) && stops(rules, above + equal, mass_above + equal * each))
-                        sh.above = above, sh.mass_above = mass_above, sh.in = equal, sh.cut = l;  // (equal ones write the same)
+#pragma unroll
+                    for (int o = 4; o > 0; o >>= 1) {
+                        above += __shfl_xor_sync(0xffffffffu, above, o);
+                        equal += __shfl_xor_sync(0xffffffffu, equal, o);
+                        mass_above += __shfl_xor_sync(0xffffffffu, mass_above, o);
+                    }
+                    above += rules.above, mass_above += rules.mass_above;
+                    if (e < rules.in && (tid & 7) == 0) {
+                        const u64 each = sh.list_m[e];
+                        if (!stops(rules, above, mass_above) && stops(rules, above + equal, mass_above + equal * each))
+                            for (int r = shared ? 0 : c; r < (shared ? C : c + 1); ++r) {  // (equal ones write the same)
+                                Sh& to = *cluster.map_shared_rank(&sh, r);
+                                to.above = above, to.mass_above = mass_above, to.in = equal, to.cut = l;
+                            }
+                    }
                 }
-                __syncthreads();
+                if (shared) cluster.sync();
+                else __syncthreads();
                 rules.above = sh.above, rules.mass_above = sh.mass_above, rules.in = sh.in;
                 cut = sh.cut;
             } else if (bin >= 0 && rules.in > 1) {
