@@ -21,8 +21,8 @@
 //
 // The row is read once (64 rows of 151,936: 39 MB, 6 us at the memory's rate), but every logit costs a mass, a
 // histogram's atomics with a cut, and a place in a running sum: instructions bound it, and with few rows the
-// cluster's barriers.  Rows of 151,936: one with top-p 15 to 22 us, eight without a cut 11, 64 with all kinds of cuts 57;
-// 256 rows of 32,003 with all three 54.
+// cluster's barriers.  Rows of 151,936: one with top-p 15 to 22 us, eight without a cut 11, 64 with all kinds of cuts 64;
+// 256 rows of 32,003 with all three 60.
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_rows_kernel(co
                     sh.list_m[i] = rules.p_on ? scale.mass(scale.template at<WIDE>(sh.list[i]), sh.table) : 0ull;
                 __syncthreads();
                 // (more than 64 comparisons a thread: each CTA takes its share and tells the others, one more meeting of
-                // 1.7 us; 64 rows of 151,936 with all kinds of cuts took 67 us on average where it now takes 57)
+                // 1.7 us; 64 rows of 151,936 with all kinds of cuts took 67 us on average where it now takes 57, logits in L2)
                 const bool shared = C > 1 && rules.in * rules.in > 64 * THREADS;
                 const int step = shared ? C : 1, mine = shared ? c : 0;
                 for (int e0 = 0; e0 < rules.in; e0 += step * (THREADS / 8)) {

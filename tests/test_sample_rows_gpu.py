@@ -195,3 +195,21 @@ def test_refusals():
         ops.sample_rows(l.cpu(), T, u)
     with pytest.raises(ops.CudaError):
         ops.sample_rows(l, T.cpu(), u)
+
+
+@pytest.mark.parametrize("B", [2, 6, 70])  # clusters of 16, of 8, and two CTAs an SM
+@pytest.mark.parametrize("many", [60, 130, 200, 270, 512, 513, 1000, 1025, 3000])
+def test_a_cut_among_many_entries_of_a_bin(many, B):
+    """So many logits within an eighth of 1/32 octave, a third of them of a few equal values, and the cut among them."""
+    V = 40000
+    rng = np.random.default_rng(many + B)
+    l = np.full((B, V), -12.0, np.float32) + rng.uniform(0, 1, (B, V)).astype(np.float32)
+    for b in range(B):
+        at = rng.permutation(V)[:many + 3]
+        near = rng.uniform(-2.0, -1.9973, many).astype(np.float32)
+        near[: many // 3] = near[rng.integers(0, 7, many // 3)]
+        l[b, at] = np.concatenate([near, np.float32([0.0, 0.1, 0.2])])
+    u = np.floor(rng.uniform(0, 1, B) * 2 ** 24) / 2 ** 24
+    check(l, [1.0] * B, u, [int(v) for v in rng.integers(4, many + 3, B)])
+    check(l, [1.0] * B, u, None, list(rng.uniform(0.3, 0.95, B)))
+    check(l, [1.0] * B, u, [int(v) for v in rng.integers(4, many + 3, B)], list(rng.uniform(0.3, 0.95, B)), [0.05] * B)
