@@ -4,9 +4,8 @@
 //    come by TMA, and so do the tile's where they follow one another (a prompt's); other tiles (where two prompts
 //    of one adapter meet, decoding rows by the hundred) are brought by four warps with 16-byte asynchronous copies
 //    straight into the operand's swizzled layout.  K goes in up to eight pieces while that fills the GPU, a tile's
-//    pieces are a cluster, and their sums meet in distributed shared memory, in order.  v goes to memory in two
-//    bfloat16 parts (16 bits: its error is 2^-9 of the result's rounding to bfloat16; three parts for a 32-bit
-//    result).  x is read once, A once a tile from the L2 cache.  8,192 rows by 4,096, three parts of rank 64: 30 to
+//    pieces are a cluster, and their sums meet in distributed shared memory, in order.  v goes to memory in
+//    three bfloat16 parts (24 bits; large ranks of a bfloat16 result: two, see splits_of).  x is read once, A once a tile from the L2 cache.  8,192 rows by 4,096, three parts of rank 64: 30 to
 //    36 us where x alone would take 10; 2,047 rows by 12,288, rank 32: 25 us (x alone: 8).  What a block does once
 //    bounds it, the barriers, the pieces' meeting and the parts' stores, beside A's way out of the cache.
 //  * up: out = base + scale B v, 128 rows by up to 4,096 of one part's columns.  v comes by TMA as the operand that it
@@ -548,6 +547,9 @@ int pieces_of(int K, int subs, int max_tiles) {
 // them B and base's groups find room for eight of a bfloat16 result, six of a 32-bit one.
 constexpr size_t MOST_SMEM = 226 * 1024;
 int v_blocks(const Args& p, int splits) { return splits * (p.parts.woven ? 2 : 1) * ((p.rank + BK - 1) / BK); }
+// The parts in which v goes from one product to the other: three (24 bits) wherever they find room, ranks to 128 (woven: to
+// 64); a bfloat16 result of larger ranks has two (16 bits: v is off by 2^-17 of itself at most, 2^-9 of the result's own rounding).
+int splits_of(const Args& p, int dt_out) { return dt_out == RFX_DT_F32 || v_blocks(p, 3) <= 6 ? 3 : 2; }
 
 template <typename TO, int SPLITS, bool WOVEN>
 int up(const Args& p, int* err, cudaStream_t s) {
@@ -605,8 +607,9 @@ namespace adapters {
 // the low-rank rows in shared memory.
 bool prompt_takes(const Args& p, int dt_out) {
     const size_t align = (size_t)p.x | (size_t)p.a | (size_t)p.b | (size_t)(p.ld_x * 2) | (size_t)(p.lda * 2);
+    const int splits = splits_of(p, dt_out);
     return p.tile == TILE && (align & 15) == 0 && p.K % 8 == 0 && p.K >= BK && p.lda == p.K && p.rank % 16 == 0 &&
-           p.parts.n * p.rank <= MAX_W && v_blocks(p, dt_out == RFX_DT_F32 ? 3 : 2) <= (dt_out == RFX_DT_F32 ? 6 : 8) && p.N <= 65535 * 64;
+           p.parts.n * p.rank <= MAX_W && v_blocks(p, splits) <= (splits == 3 ? 6 : 8) && p.N <= 65535 * 64;
 }
 
 long long prompt_low_floats(int R, int W) { return ((long long)3 * R * W + 1) / 2; }  // three bfloat16 parts at most
@@ -628,11 +631,12 @@ int prompt_form(const Args& p, int dt_out, int* err, cudaStream_t s) {
     static SmemLimit limit;
     cudaError_t e = limit.raise(adapter_low_tc_kernel, smem);
     if (e != cudaSuccess) return (int)e;
-    const bool wide = dt_out == RFX_DT_F32;
+    const int splits = splits_of(p, dt_out);
     e = launch(adapter_low_tc_kernel, dim3(p.max_tiles, 1, pieces), LOW_THREADS, smem, s, pieces, p, map_a, map_x, box, subs, stages,
-               wide ? 3 : 2, cols, err);
+               splits, cols, err);
     if (e != cudaSuccess) return (int)e;
-    if (wide) return p.parts.woven ? up<float, 3, true>(p, err, s) : up<float, 3, false>(p, err, s);
+    if (dt_out == RFX_DT_F32) return p.parts.woven ? up<float, 3, true>(p, err, s) : up<float, 3, false>(p, err, s);
+    if (splits == 3) return p.parts.woven ? up<__nv_bfloat16, 3, true>(p, err, s) : up<__nv_bfloat16, 3, false>(p, err, s);
     return p.parts.woven ? up<__nv_bfloat16, 2, true>(p, err, s) : up<__nv_bfloat16, 2, false>(p, err, s);
 }
 
