@@ -29,6 +29,7 @@ using namespace adapters;
 using namespace sm100;
 
 constexpr int TILE = 128, BK = 64, LOW_THREADS = 384, MAX_STAGES = 8, MAX_W = 512, CHUNK = 256, MAX_PIECES = 8;
+constexpr int MAX_SUMS = 4;  // accumulators that take turns
 constexpr int X_BYTES = TILE * BK * 2;
 
 // Stages, of `subs` blocks of 64 along K, that each of `pieces` takes.
@@ -60,7 +61,7 @@ __device__ __forceinline__ void store_parts(__nv_bfloat16* dst, size_t apart, in
 __global__ void __launch_bounds__(LOW_THREADS)
 adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
                       const __grid_constant__ CUtensorMap map_x, int box, int subs, int stages, int splits,
-                      uint32_t tmem_cols, int* __restrict__ err) {
+                      uint32_t tmem_cols, int turns, int* __restrict__ err) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], done_bar;
     __shared__ uint32_t tmem_base;
@@ -98,7 +99,7 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
     __syncthreads();
     tc_fence_after_sync();
     pdl_launch_dependents();  // (not before tensor memory is this block's: the next kernel's blocks would take it)
-    const uint32_t tmem = tmem_base;
+    const uint32_t tmem = tmem_base, apart = tmem_cols / turns;  // `turns` accumulators, a stage each in turn
     bool ok = true;
     if (warp < 4) {
         auto bring = [&](int s, int k) {  // A's rows of all parts, and the tile's where they follow one another
@@ -162,8 +163,7 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
             const uint32_t stage_step = (uint32_t)stage_bytes >> 4;
             const uint32_t idesc = umma_idesc_bf16(TILE, min(256, W)), idesc2 = umma_idesc_bf16(TILE, max(16, W - 256));
             uint64_t dx = desc0;
-            uint32_t more = 0;
-            int s = 0, ph = 0;
+            int s = 0, ph = 0, turn = 0;
             for (int i = 0; i < nkb; ++i) {
                 if (!mbar_wait(&full_bar[s], ph)) {
                     atomicExch(err, 63);
@@ -173,12 +173,15 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
                 // rows brought by threads were written by the generic proxy; the tensor cores read by the asynchronous one
                 if (!run) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 tc_fence_after_sync();
+                const uint32_t d = tmem + turn * apart;
+                uint32_t more = i >= turns;
+                if (++turn == turns) turn = 0;
                 for (int b = 0; b < subs; ++b) {
                     const uint64_t db = dx + b * (X_BYTES / 16), da = dx + subs * (X_BYTES / 16) + b * (W * 8);
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k) {
-                        umma_bf16(tmem, db + 2 * k, da + 2 * k, idesc, more);
-                        if (W > 256) umma_bf16(tmem + 256, db + 2 * k, da + 256 * 8 + 2 * k, idesc2, more);
+                        umma_bf16(d, db + 2 * k, da + 2 * k, idesc, more);
+                        if (W > 256) umma_bf16(d + 256, db + 2 * k, da + 256 * 8 + 2 * k, idesc2, more);
                         more = 1;
                     }
                 }
@@ -206,6 +209,12 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
             for (int c = 0; c < wide; c += 16) {
                 float v[16];
                 tmem_ld_16(tmem + ((uint32_t)(warp * 32) << 16) + c0 + c, v);
+                for (int q = 1; q < min(turns, nkb); ++q) {
+                    float u[16];
+                    tmem_ld_16(tmem + ((uint32_t)(warp * 32) << 16) + q * apart + c0 + c, u);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] += u[j];
+                }
                 if (row < t.count)
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) store4(dst + c + j, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
@@ -473,7 +482,7 @@ adapter_up_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_v, in
                     const uint32_t d = tmem_base + (i & 1) * cols + q * (cols / 2);
                     uint32_t more = 0;
 #pragma unroll
-                    for (int sp = 0; sp < SPLITS; ++sp) {
+                    for (int sp = SPLITS - 1; sp >= 0; --sp) {  // the smallest first: what is cut off is small as well
                         uint64_t dv = desc_v + (uint32_t)((sp * PARTS + q) * kb) * (X_BYTES / 16), db = db0 + q * (cols / 2) * 8;
                         for (int k = 0; k < steps; ++k) {
                             umma_bf16(d, dv, db, idesc, more);
@@ -627,13 +636,15 @@ int prompt_form(const Args& p, int dt_out, int* err, cudaStream_t s) {
     if (stages > 6) stages = 6;
     uint32_t cols = 32;
     while ((int)cols < W) cols *= 2;
+    // A tensor core cuts sums off, always towards zero: accumulators that take turns keep the chains short
+    const int turns = (int)min((uint32_t)MAX_SUMS, 512 / cols);
     const size_t smem = (size_t)stages * stage + 1024;
     static SmemLimit limit;
     cudaError_t e = limit.raise(adapter_low_tc_kernel, smem);
     if (e != cudaSuccess) return (int)e;
     const int splits = splits_of(p, dt_out);
     e = launch(adapter_low_tc_kernel, dim3(p.max_tiles, 1, pieces), LOW_THREADS, smem, s, pieces, p, map_a, map_x, box, subs, stages,
-               splits, cols, err);
+               splits, cols * turns, turns, err);
     if (e != cudaSuccess) return (int)e;
     if (dt_out == RFX_DT_F32) return p.parts.woven ? up<float, 3, true>(p, err, s) : up<float, 3, false>(p, err, s);
     if (splits == 3) return p.parts.woven ? up<__nv_bfloat16, 3, true>(p, err, s) : up<__nv_bfloat16, 3, false>(p, err, s);

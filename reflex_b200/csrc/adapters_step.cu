@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, 
         for (int n = warp; n < tiles; n += WARPS) {
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
             for (int i = 0; i < blocks; i += BATCH) {
+                float some[4] = {0.f, 0.f, 0.f, 0.f};  // a batch's: the tensor cores cut sums off, and chains are kept short
                 bring();
                 attn::cp_async_wait<RING - 1>();
                 uint4 w[BATCH], xa[BATCH], xb[BATCH];
@@ -199,9 +200,11 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, 
 #pragma unroll
                 for (int j = 0; j < BATCH; ++j) {
                     const uint32_t f0[4] = {xa[j].x, xb[j].x, xa[j].y, xb[j].y}, f1[4] = {xa[j].z, xb[j].z, xa[j].w, xb[j].w};
-                    attn::mma_bf16(acc, f0, w[j].x, w[j].y);
-                    attn::mma_bf16(acc, f1, w[j].z, w[j].w);
+                    attn::mma_bf16(some, f0, w[j].x, w[j].y);
+                    attn::mma_bf16(some, f1, w[j].z, w[j].w);
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] += some[j];
             }
             if (push) {
 #pragma unroll
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_step_kernel(const Args p, 
             if (++slot == RING) slot = 0;
             const bool there = i * 32 + t * 8 < per * 8;  // (what lies beyond is no number of this part)
 #pragma unroll
-            for (int q = 0; q < 3; ++q) {
+            for (int q = 2; q >= 0; --q) {  // the smallest part first
                 auto frag = [&](int sp, uint4& lo, uint4& hi) {
                     const uint32_t at = v_at + (q * TILE * LDV + sp * per * 8 + i * 32) * 2;
                     lo = hi = make_uint4(0, 0, 0, 0);
