@@ -298,6 +298,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_rows_kernel(co
     float* piece = reinterpret_cast<float*>(dynamic) + 3 * BINS;
     if (tid < PER_OCTAVE) sh.table[tid] = exp2((double)-tid / PER_OCTAVE);
     if (tid == 0) sh.listed = 0;
+    cluster.barrier_arrive();  // met below: every CTA has begun before another writes into its memory
     pdl_prologue();
     const size_t b = blockIdx.x;
     const int lo = min(p.V, c * p.chunk), n = min(p.V, lo + p.chunk) - lo;
@@ -331,6 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_rows_kernel(co
     if (lane == 0) sh.warp_f[warp] = mx;
     __syncthreads();
     for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, sh.warp_f[w]);
+    cluster.barrier_wait();
     tell_all(cluster, sh.top, mx);
     for (int i = 0; i < C; ++i) mx = fmaxf(mx, sh.top[i]);
     if (mx == -INFINITY) {  // nothing left
