@@ -635,6 +635,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_rows_kernel(co
 
 }  // namespace
 
+// CTAs a row.  A cluster of 16 halves what its CTAs have to go over (a row of 151,936 with top-p: 23 -> 20 us), but a
+// group of SMs holds one: eight rows took 16 us where clusters of eight take 11.  Only CTAs that each have an SM to
+// themselves have room for what sixteen exchange.
+extern "C" int rfx_sample_rows_ctas(int B, int V, int sms) {
+    const int most = B <= 4 && 16 * B <= sms ? 16 : 8;
+    int C = 1;
+    while (C < most && (long long)C * 4096 < V && ((long long)B * C < 2 * sms || (long long)C * 19200 < V)) C *= 2;
+    return C;
+}
+
 // temperature [B] (<= 0 or NaN: greedy), uniform [B] in [0, 1); top_k (<= 0 or >= V: off), top_p (>= 1: off)
 // and min_p (<= 0: off, above 1 as 1) [B] or null.
 extern "C" int rfx_sample_rows(const float* logits, long long ld, int B, int V, const float* temperature,
@@ -642,11 +652,7 @@ extern "C" int rfx_sample_rows(const float* logits, long long ld, int B, int V, 
                                void* stream) {
     if (B <= 0) return 0;
     if (V <= 0 || ld < V) return RFX_ERR_BAD_ARG;
-    // A cluster of 16 halves what its CTAs have to go over (a row of 151,936 with top-p: 23 -> 20 us), but a group of SMs
-    // holds one: eight rows took 16 us where clusters of eight take 11.
-    const int most = B <= 4 ? 16 : 8;
-    int C = 1;
-    while (C < most && (long long)C * 4096 < V && ((long long)B * C < 2 * sm_count() || (long long)C * 19200 < V)) C *= 2;
+    const int C = rfx_sample_rows_ctas(B, V, sm_count());
     const int chunk = ((V + C - 1) / C + 3) / 4 * 4;
     const size_t hist = (size_t)BINS * 12, piece = (size_t)chunk * 4;
     const bool staged = hist + piece <= 200 * 1024;

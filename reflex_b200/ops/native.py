@@ -216,6 +216,7 @@ _SIGNATURES = {
     "rfx_argmax": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "rfx_sample_rows": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                         c_void_p],
+    "rfx_sample_rows_ctas": [c_int, c_int, c_int],
     "rfx_adapter_rows": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
     "rfx_adapter_form": [c_void_p, c_int, c_int],
     "rfx_adapter_add": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int,
