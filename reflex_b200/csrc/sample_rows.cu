@@ -178,7 +178,7 @@ struct Rules {
     int k;          // 0: no top-k
     bool p_on;
     float p;
-    u64 want;       // top_p times the whole mass
+    u64 want;       // top_p times the whole mass, one unit at least: the first token is kept whatever top_p is
     int above;
     u64 mass_above;
     int in;         // entries in the bin last chosen
@@ -233,7 +233,7 @@ __device__ int choose(cg::cluster_group& cluster, Sh& sh, const Hist& hist, Rule
         if (totals && rules.p_on) {
             u64 all = __shfl_sync(0xffffffffu, im, 31);
             for (int r = 0; r < C; ++r) all += sh.far[r];
-            rules.want = (u64)ceil((double)rules.p * (double)all);
+            rules.want = max((u64)ceil((double)rules.p * (double)all), 1ull);
             if (lane == 0) sh.total = all;
         }
         // two coarse bins a lane
@@ -251,7 +251,7 @@ __device__ int choose(cg::cluster_group& cluster, Sh& sh, const Hist& hist, Rule
         }
     }
     __syncthreads();
-    if (totals && rules.p_on) rules.want = (u64)ceil((double)rules.p * (double)sh.total);
+    if (totals && rules.p_on) rules.want = max((u64)ceil((double)rules.p * (double)sh.total), 1ull);
     const int q = sh.bin;
     if (q < 0) return q;
     // the 32 bins of the chosen one, a warp a CTA
