@@ -100,7 +100,6 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
     tc_fence_after_sync();
     pdl_launch_dependents();  // (not before tensor memory is this block's: the next kernel's blocks would take it)
     const uint32_t tmem = tmem_base, apart = tmem_cols / turns;  // `turns` accumulators, a stage each in turn
-    bool ok = true;
     if (warp < 4) {
         auto bring = [&](int s, int k) {  // A's rows of all parts, and the tile's where they follow one another
             uint8_t *dst = stage0 + (size_t)s * stage_bytes, *a = dst + subs * X_BYTES;
@@ -119,7 +118,6 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
                 for (int i = 0; i < nkb; ++i) {
                     if (i >= stages && !mbar_wait(&empty_bar[s], ph)) {
                         atomicExch(err, 61);
-                        ok = false;
                         break;
                     }
                     bring(s, (kb0 + i) * step);
@@ -133,7 +131,6 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
             for (int i = 0; i < nkb; ++i) {
                 if (i >= stages && !mbar_wait(&empty_bar[s], ph)) {
                     atomicExch(err, 61);
-                    ok = false;
                     break;
                 }
                 uint8_t* dst = stage0 + (size_t)s * stage_bytes;
@@ -153,7 +150,10 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
             }
             attn::cp_async_wait<0>();
         }
-        if (!mbar_wait(&done_bar, 0)) atomicExch(err, 62);
+        if (!mbar_wait(&done_bar, 0)) {
+            atomicExch(err, 62);
+            mbar_wait(&done_bar, 0);  // as long again for what is still being multiplied
+        }
         tc_fence_after_sync();
         __syncwarp();
     } else if (warp == 4) {
@@ -167,7 +167,8 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
             for (int i = 0; i < nkb; ++i) {
                 if (!mbar_wait(&full_bar[s], ph)) {
                     atomicExch(err, 63);
-                    ok = false;
+                    // nothing more is begun; the stages that may still be on their way get as long again each
+                    for (int j = i; j < min(nkb, i + stages); ++j) mbar_wait(&full_bar[j % stages], j / stages & 1);
                     break;
                 }
                 // rows brought by threads were written by the generic proxy; the tensor cores read by the asynchronous one
@@ -189,7 +190,7 @@ adapter_low_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_a,
                 dx += stage_step;
                 if (++s == stages) s = 0, ph ^= 1, dx = desc0;
             }
-            if (ok) umma_commit(&done_bar);
+            umma_commit(&done_bar);  // (after a wait that ran out too: for the products before it)
         }
         __syncwarp();
     }
@@ -466,11 +467,16 @@ adapter_up_tc_kernel(const Args p, const __grid_constant__ CUtensorMap map_v, in
             const uint32_t idesc = umma_idesc_bf16(TILE, cols / PARTS), b_step = (uint32_t)(kb * cols * 8);
             const uint64_t desc_v = umma_desc_k_sw128(smem_u32(vs)), desc_b = umma_desc_k_sw128(smem_u32(bs));
             int s = 0, ph = 0;
-            bool ok = mbar_wait(&v_full, 0);
-            if (!ok) atomicExch(err, 67);
+            const bool ok = mbar_wait(&v_full, 0);
+            if (!ok) {
+                atomicExch(err, 67);
+                mbar_wait(&v_full, 0);  // as long again for the copies on their way
+            }
             for (int i = 0; i < turns && ok; ++i) {
                 if ((i >= 2 && !mbar_wait(&acc_empty[i & 1], (i >> 1 & 1) ^ 1)) || !mbar_wait(&b_full[s], ph)) {
                     atomicExch(err, 65);
+                    // nothing more is begun; the products on their way get as long again
+                    for (int j = max(i - 2, 0); j < i; ++j) mbar_wait(&acc_full[j & 1], j >> 1 & 1);
                     break;
                 }
                 // B's columns were written by the generic proxy; the tensor cores read by the asynchronous one
