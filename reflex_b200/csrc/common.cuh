@@ -10,6 +10,7 @@
 #include <utility>
 
 #include "exact_math.cuh"
+#include "smem_limit.h"
 
 #define RFX_DT_F32 0
 #define RFX_DT_BF16 1
@@ -67,30 +68,6 @@ inline int sm_count() {
     }
     return n;
 }
-
-// The dynamic shared memory that one kernel may ask for, raised when a launch asks for more than any before
-// it, and, where asked for, clusters of more than eight blocks: one static object a kernel, so that a call does not
-// pay for the attributes again.
-struct SmemLimit {
-    int have[16] = {};
-    bool wide[16] = {};
-    template <typename K>
-    cudaError_t raise(K kernel, size_t bytes, bool wide_clusters = false) {
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess) return e;
-        int* h = dev >= 0 && dev < 16 ? &have[dev] : nullptr;
-        if (wide_clusters && !(h && wide[dev])) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-            if (e != cudaSuccess) return e;
-            if (h) wide[dev] = true;
-        }
-        if (h && *h >= (int)bytes) return cudaSuccess;
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e == cudaSuccess && h) *h = (int)bytes;
-        return e;
-    }
-};
 
 // Launch with the library's attributes; cluster_z > 1 asks for a thread-block
 // cluster of (1, 1, cluster_z).
