@@ -107,7 +107,6 @@ class Model:
         self.max_batch = max_batch
         self.engine = Engine(causal_lm, max_tokens=max_tokens, use_graphs=use_graphs)
         self.last_stats: Optional[GenerationStats] = None
-        self.adapter_names: List[str] = []
         # the generation loop keeps the device one step ahead of the host
         self.decode_ahead = True
 
@@ -138,8 +137,12 @@ class Model:
         from .weights.adapters import read_adapter
 
         read = [read_adapter(folder, self.spec) for folder in folders.values()]
-        self.engine.load_adapters(read)
-        self.adapter_names = list(folders)
+        self.engine.load_adapters(read, list(folders))
+
+    @property
+    def adapter_names(self) -> List[str]:
+        """The loaded adapters, in the order of their numbers (the weights' own: every `Model` of them has the same)."""
+        return list(self.lm.adapter_names)
 
     def adapter(self, name: str) -> int:
         """The number of a loaded adapter, as `Engine.open` takes it."""

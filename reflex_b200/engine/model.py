@@ -8,6 +8,7 @@ holds parts and weights; what a step changes lives in the cache and the batch.
 
 from __future__ import annotations
 
+import weakref
 from dataclasses import dataclass
 from typing import Any, Dict, List, Optional, Tuple
 
@@ -85,6 +86,8 @@ class CausalLM:
         # a probe for tests and diagnostics: called after every layer run with (index,
         # run, layer, hidden, pending); None in normal use
         self.after_run = None
+        # the engines that run it: what is open and captured there goes by the adapters bound here
+        self.engines = weakref.WeakSet()
         if any(r.mixes_input for r in spec.run_order) and spec.stream_mix_name is None:
             raise ValueError("a run mixes its input but the model names no stream-mix matrix")
         if any(r.pass_vector is not None for r in spec.run_order) and spec.pass_vectors_name is None:
@@ -136,10 +139,11 @@ class CausalLM:
             self.head = self.embedding  # the same storage, no copy
 
     n_adapters = 0
+    adapter_names: Tuple[str, ...] = ()
 
-    def bind_adapters(self, adapters) -> None:
-        """`adapters`: what `weights.adapters.read_adapter` gave for each; they take the place of those bound before.
-        Nothing changes where one of them names a matrix that its part does not take adapters for."""
+    def bind_adapters(self, adapters, names=()) -> None:
+        """`adapters`: what `weights.adapters.read_adapter` gave for each, and their names where they have any; they
+        take the place of those bound before (`Engine.load_adapters` sees to the engines that run the model).  Nothing changes where one of them names a matrix that its part does not take adapters for."""
         exp = expected_tensors(self.spec)
         parts: Dict[Tuple[int, str], Dict[str, list]] = {}
         for i, adapter in enumerate(adapters):
@@ -160,7 +164,7 @@ class CausalLM:
                     made.append((part, part.adapter_banks(parts.get((li, name), {}), scales)))
         for part, banks in made:
             part.adapters = banks
-        self.n_adapters = len(adapters)
+        self.n_adapters, self.adapter_names = len(adapters), tuple(names)
 
     # --- cache ------------------------------------------------------------
     def cache_entry_specs(self) -> Dict[int, Any]:

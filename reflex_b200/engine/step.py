@@ -41,6 +41,7 @@ class Engine:
     def __init__(self, model: CausalLM, max_tokens: int, max_slots: Optional[int] = None,
                  use_graphs: bool = True, max_graphs: int = 48):
         self.model = model
+        model.engines.add(self)
         self.device = model.device
         self.cache = Cache(model.cache_entry_specs(), max_tokens, model.spec.max_positions,
                            model.dtype, model.device, max_slots=max_slots)
@@ -80,15 +81,17 @@ class Engine:
         self.cache.give_slot(seq)
         self._adapter_of.pop(seq, None)
 
-    def load_adapters(self, adapters) -> None:
+    def load_adapters(self, adapters, names=()) -> None:
         """The model's adapters from now on, in place of earlier ones (`CausalLM.bind_adapters`); no sequence may be
-        open that uses one."""
-        if self._adapter_of:
+        open that uses one, in this engine or another of the same model."""
+        every = list(self.model.engines)
+        if any(e._adapter_of for e in every):
             raise InvalidInput("adapters cannot be exchanged while sequences that use them are open")
         if torch.device(self.device).type == "cuda":
             torch.cuda.synchronize(self.device)  # a step that reads the earlier ones may still run
-        self._graphs = {k: g for k, g in self._graphs.items() if not k[2]}  # captured steps point at the earlier ones
-        self.model.bind_adapters(adapters)
+        for e in every:  # captured steps point at the earlier ones
+            e._graphs = {k: g for k, g in e._graphs.items() if not k[2]}
+        self.model.bind_adapters(adapters, names)
 
     def _row_adapters(self, slots, counts=None):
         """The adapter of every row of a step, -1 for none (NumPy int32); None where no sequence has one."""
