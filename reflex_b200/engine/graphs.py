@@ -77,11 +77,14 @@ class DecodeGraph:
             # Beyond the rows the library's own products take, the step calls the
             # vendor's matrix product, which picks (and loads) a kernel per shape the
             # first time it sees it, and loading inside a capture invalidates it: such
-            # a batch size runs eagerly once before it is captured.
-            first_of_size = self.n > ops.GEMV_MAX_ROWS and self.n not in eng._eager_sizes
+            # a batch size runs eagerly once before it is captured, and once more with
+            # adapters, beside which other products are called (results of their own
+            # where the plain step adds to the stream).
+            size = self.n, self.adapter_ids is not None
+            first_of_size = self.n > ops.GEMV_MAX_ROWS and size not in eng._eager_sizes
             if eng._eager_decodes < self.WARMUP or first_of_size:
                 eng._eager_decodes += 1
-                eng._eager_sizes.add(self.n)
+                eng._eager_sizes.add(size)
                 return self._forward(batch)
             # capture: the eager call above has already sized every lazy buffer
             torch.cuda.synchronize()

@@ -57,7 +57,7 @@ class Engine:
         self._adapter_of: Dict[int, int] = {}  # sequences that go through one of the model's adapters
         self._graph_pool = None
         self._eager_decodes = 0  # eager decode steps run so far
-        self._eager_sizes: set = set()  # batch sizes that have run eagerly once
+        self._eager_sizes: set = set()  # (sequences, with adapters) that have run eagerly once
         self.steps_run = 0
         on_gpu = torch.device(self.device).type == "cuda"
         self.staging = Staging(self.device) if on_gpu else None
