@@ -104,8 +104,8 @@ __global__ void rmsnorm_kernel(const float* x, const TD* __restrict__ delta,
 // out[r, i] = act(gate_i) * up_i, act silu, g / (1 + exp(-g)), or (ACT 1) the tanh form of gelu
 // (src/kernels_cuda/silu_and_mul.cu:7-23).  A row of `gu` holds the gates in its
 // first half and the ups in its second, or (alternating) gate_i at 2i, up_i at 2i+1.
-template <typename T, int ACT>
-__global__ void swiglu_kernel(const T* __restrict__ gu, T* __restrict__ out, int R, int I,
+template <typename T, typename TO, int ACT>
+__global__ void swiglu_kernel(const T* __restrict__ gu, TO* __restrict__ out, int R, int I,
                               int alternating) {
     pdl_prologue();
     const size_t n = (size_t)R * I;
@@ -114,7 +114,7 @@ __global__ void swiglu_kernel(const T* __restrict__ gu, T* __restrict__ out, int
         const size_t r = i / I, c = i % I;
         const float g = ld<T>(gu, r * 2 * I + (alternating ? 2 * c : c));
         const float u = ld<T>(gu, r * 2 * I + (alternating ? 2 * c + 1 : I + c));
-        st<T>(out, i, gated_mul_for<T, ACT>(g, u));
+        st<TO>(out, i, gated_mul_for<TO, ACT>(g, u));
     }
 }
 
@@ -253,8 +253,9 @@ extern "C" int rfx_rmsnorm(const float* x, const void* delta, int delta_dt, floa
     return 0;
 }
 
-// `act`: 0 silu, 1 the tanh form of gelu.
-extern "C" int rfx_gated_act(const void* gate_up, void* out, int dt, int R, int I, int alternating, int act,
+// `act`: 0 silu, 1 the tanh form of gelu.  `out_dt` is `dt`, or bfloat16 beside 32-bit sums (as a product's own
+// epilogue has them).
+extern "C" int rfx_gated_act(const void* gate_up, void* out, int dt, int out_dt, int R, int I, int alternating, int act,
                              void* stream) {
     if (R <= 0 || I <= 0) return 0;
     if (act != 0 && act != 1) return RFX_ERR_BAD_ARG;
@@ -262,15 +263,18 @@ extern "C" int rfx_gated_act(const void* gate_up, void* out, int dt, int R, int 
     const size_t n = (size_t)R * I;
     int blocks = (int)((n + 255) / 256);
     if (blocks > sm_count() * 16) blocks = sm_count() * 16;
-#define RFX_GO(T)                                                                                                \
-    do {                                                                                                         \
-        if (act == 0)                                                                                            \
-            RFX_LAUNCH((swiglu_kernel<T, 0>), blocks, 256, 0, s, (const T*)gate_up, (T*)out, R, I, alternating); \
-        else                                                                                                     \
-            RFX_LAUNCH((swiglu_kernel<T, 1>), blocks, 256, 0, s, (const T*)gate_up, (T*)out, R, I, alternating); \
+    if (dt != out_dt && !(dt == RFX_DT_F32 && out_dt == RFX_DT_BF16)) return RFX_ERR_BAD_ARG;
+#define RFX_GO(T, TO)                                                                                                 \
+    do {                                                                                                              \
+        if (act == 0)                                                                                                 \
+            RFX_LAUNCH((swiglu_kernel<T, TO, 0>), blocks, 256, 0, s, (const T*)gate_up, (TO*)out, R, I, alternating); \
+        else                                                                                                          \
+            RFX_LAUNCH((swiglu_kernel<T, TO, 1>), blocks, 256, 0, s, (const T*)gate_up, (TO*)out, R, I, alternating); \
     } while (0)
-    if (dt == RFX_DT_F32) {
-        RFX_GO(float);
+    if (dt == RFX_DT_F32 && out_dt == RFX_DT_BF16) {
+        RFX_GO(float, __nv_bfloat16);
+    } else if (dt == RFX_DT_F32) {
+        RFX_GO(float, float);
     } else if (dt == RFX_DT_BF16 && I % 8 == 0 &&
                ((reinterpret_cast<uintptr_t>(gate_up) | reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
         int b8 = (int)((n / 8 + 255) / 256);
@@ -282,7 +286,7 @@ extern "C" int rfx_gated_act(const void* gate_up, void* out, int dt, int R, int 
             RFX_LAUNCH(swiglu_bf16x8_kernel<1>, b8, 256, 0, s, (const __nv_bfloat16*)gate_up, (__nv_bfloat16*)out, R,
                        I, alternating);
     } else if (dt == RFX_DT_BF16) {
-        RFX_GO(__nv_bfloat16);
+        RFX_GO(__nv_bfloat16, __nv_bfloat16);
     } else {
         return RFX_ERR_BAD_ARG;
     }
@@ -291,7 +295,7 @@ extern "C" int rfx_gated_act(const void* gate_up, void* out, int dt, int R, int 
 }
 
 extern "C" int rfx_swiglu(const void* gate_up, void* out, int dt, int R, int I, int alternating, void* stream) {
-    return rfx_gated_act(gate_up, out, dt, R, I, alternating, 0, stream);
+    return rfx_gated_act(gate_up, out, dt, dt, R, I, alternating, 0, stream);
 }
 
 extern "C" int rfx_add(float* a, const void* b, int b_dt, long long n, void* stream) {

@@ -104,15 +104,19 @@ def add_(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
 GATED_ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
 
 
-def swiglu(gate_up: torch.Tensor, alternating: bool = False, activation: str = "silu") -> torch.Tensor:
+def swiglu(gate_up: torch.Tensor, alternating: bool = False, activation: str = "silu",
+           out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """[R, 2I] -> act(gate) * up, [R, I], act silu or the tanh form of gelu.  A row holds the gates in its first
     half and the ups in its second, or (`alternating`) gate_i at 2i and up_i at
-    2i + 1."""
+    2i + 1.  The result has `gate_up`'s type; that of 32-bit sums may be bfloat16 (`out_dtype`)."""
     R, two_i = gate_up.shape
     I = two_i // 2
-    out = _new((R, I), gate_up.dtype, gate_up.device)
+    out_dtype = out_dtype or gate_up.dtype
+    if out_dtype != gate_up.dtype and (gate_up.dtype, out_dtype) != (torch.float32, torch.bfloat16):
+        raise InvalidInput(f"swiglu: {gate_up.dtype} does not go to {out_dtype}")
+    out = _new((R, I), out_dtype, gate_up.device)
     st = native.lib().rfx_gated_act(_chk(gate_up, "gate_up"), out.data_ptr(), dt_code(gate_up.dtype),
-                                    R, I, 1 if alternating else 0, GATED_ACTIVATIONS[activation], _stream())
+                                    dt_code(out_dtype), R, I, 1 if alternating else 0, GATED_ACTIVATIONS[activation], _stream())
     native.check(st, f"gated_act ({activation})")
     return out
 

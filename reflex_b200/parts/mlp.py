@@ -70,7 +70,11 @@ class SwiGLU:
         returns the delta."""
         gate_up_adapters, down_adapters = self.adapters if ops.active_adapters() is not None else (None, None)
         if gate_up_adapters is not None:
-            act = ops.swiglu(add(ops.linear(x, self.gate_up), x, gate_up_adapters), alternating=True)
+            # a decode step's sums stay in 32 bits up to the activation, as in the fused product's epilogue; a prompt's
+            # have the type that they have without adapters (rounded once more behind the adapter)
+            few = x.shape[0] <= ops.GEMV_MAX_ROWS
+            sums = add(ops.linear(x, self.gate_up, out_dtype=torch.float32 if few else None), x, gate_up_adapters)
+            act = ops.swiglu(sums, alternating=True, out_dtype=x.dtype)
         else:
             act = ops.linear_swiglu(x, self.gate_up)
         ops.prof_mark("ffn_gate_up")
