@@ -128,8 +128,8 @@ class Sampler:
         mine = [0 if len(self.every) == 1 else r for r in requests]
         rules = [self.every[i] for i in mine]
 
-        def numbers(name, off):
-            return [off if getattr(p, name) is None else getattr(p, name) for p in rules]
+        def numbers(name, off):  # (greedy parameters are not checked, nor needed)
+            return [off if p.is_greedy() or getattr(p, name) is None else getattr(p, name) for p in rules]
 
         words = np.empty((5, n), dtype=np.float32)
         words[0] = [uniform(self.seeds[i], r, s) for i, r, s in zip(mine, requests, steps)]
@@ -137,7 +137,7 @@ class Sampler:
         words[2], words[3] = numbers("top_p", 1.0), numbers("min_p", 0.0)
         words[4].view(np.int32)[:] = [min(k, logits.shape[1]) for k in numbers("top_k", 0)]
         u, t, p, m, k = self._upload(words.reshape(-1)).view(5, n)
-        has = [any(getattr(q, name) is not None for q in rules) for name in ("top_k", "top_p", "min_p")]
+        has = [any(getattr(q, name) is not None and not q.is_greedy() for q in rules) for name in ("top_k", "top_p", "min_p")]
         ops.sample_rows(logits, t, u, top_k=k.view(torch.int32) if has[0] else None, top_p=p if has[1] else None,
                         min_p=m if has[2] else None, out=out)
 
