@@ -433,6 +433,9 @@ class AdapterRows:
             raise InvalidInput(f"AdapterRows: tiles have 16 or 128 rows, not {tile}")
         if order.dim() != 1 or first.dim() != 1 or first.shape[0] < 3 or tiles.dim() != 2 or tiles.shape[1] != 3:
             raise InvalidInput("AdapterRows: order [rows], first [adapters + 2] and tiles [tiles, 3] are needed")
+        if first.device != order.device or tiles.device != order.device:
+            raise InvalidInput("AdapterRows: order, first and tiles live on one device")
+        _chk(first, "first", torch.int32)
         self._memory, self._parts, self.tile, self.index = None, (order, first, tiles), tile, order.get_device()
         self.n_rows, self.n, self.n_tiles = order.shape[0], first.shape[0] - 2, tiles.shape[0]
         self.order_ptr, self.tiles_ptr = _chk(order, "order", torch.int32), _chk(tiles, "tiles", torch.int32)
