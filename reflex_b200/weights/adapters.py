@@ -53,7 +53,7 @@ def read_adapter(folder: str, spec: ModelSpec) -> Adapter:
     if isinstance(alpha, bool) or not isinstance(alpha, (int, float)) or not abs(alpha) < 2.0 ** 127:
         raise CheckpointError(f"{path}: lora_alpha must be a number, got {alpha!r}")
     for key, off in _OFF.items():
-        if cfg.get(key, off) not in (off, None):
+        if cfg.get(key, off) not in (off, None, [], {}):
             raise UnsupportedArchitecture(f"{path}: {key} = {cfg[key]!r} is not supported")
     exp = expected_tensors(spec)
     wrong, sides = [], {}
