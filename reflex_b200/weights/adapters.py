@@ -24,7 +24,7 @@ from .safetensors_io import SafetensorsFile
 PREFIX = "base_model.model."
 # options that change more than W -> W + scale B A, and the value that leaves them off
 _OFF = {"use_dora": False, "fan_in_fan_out": False, "bias": "none", "modules_to_save": None, "rank_pattern": {},
-        "alpha_pattern": {}, "lora_bias": False, "layer_replication": None}
+        "alpha_pattern": {}, "lora_bias": False, "layer_replication": None, "alora_invocation_tokens": None}
 
 
 @dataclass

@@ -36,3 +36,10 @@ def test_options_that_are_left_off(more):
 def test_options_that_change_more(more):
     with pytest.raises(UnsupportedArchitecture, match=next(iter(more))):
         read(**more)
+
+
+def test_an_adapter_that_begins_at_certain_tokens():
+    """Rows before them go without it, which no sequence here does."""
+    with pytest.raises(UnsupportedArchitecture, match="alora_invocation_tokens"):
+        read(alora_invocation_tokens=[5, 6])
+    read(alora_invocation_tokens=None)
