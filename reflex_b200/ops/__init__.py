@@ -419,6 +419,7 @@ def linear_geglu(x: torch.Tensor, weight_pairs: torch.Tensor) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------ adapters
+ADAPTER_STEP_TILES = 65535  # that the launch for tiles of 16 takes; beyond, the products go by multiply-adds
 ADAPTER_STEP_ROWS = 256  # up to here rows go by tiles of 16, as requests that bring a token each; beyond by tiles of 128
 
 
@@ -628,6 +629,8 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, rows: Ad
             raise InvalidInput("adapter_add: out is base itself, or overlaps neither base nor x")
     xp = x.data_ptr()
     form = bank._form[rows.tile, dtype] if (xp | ld_x * 2) % 16 == 0 else 0
+    if form == 1 and rows.n_tiles > ADAPTER_STEP_TILES:
+        form = 0
     lib = native.lib()
     low = 0
     if form != 1:
