@@ -90,6 +90,8 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     __shared__ __align__(8) uint64_t empty_bar[STG];  // TMA: the four warps are done with the stage
     constexpr int NT = TMA ? DEC_THREADS + 32 : DEC_THREADS;  // TMA: a fifth warp that issues the loads
 
+    // (met before anything is sent: every rank of the cluster has begun)
+    if (n_splits > 1 && cluster_merge) rfx::cluster_begun();
     rfx::pdl_launch_dependents();
     if (TMA) {
         if (threadIdx.x == 0) {
@@ -385,6 +387,7 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         }
     }
     __syncthreads();
+    if (n_splits > 1 && cluster_merge) rfx::cluster_all_begun();
     const int total = nh * DV;
     const int slice = (total + n_splits - 1) / n_splits;  // elements of the tile's output a rank merges
     for (int i = tid; i < total; i += NT) {

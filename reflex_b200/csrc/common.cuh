@@ -69,6 +69,11 @@ inline int sm_count() {
     return n;
 }
 
+// Every thread of a cluster's blocks says that it has begun, and later waits for the others before the block writes into
+// another's shared memory; nothing is ordered by it but that.
+__device__ __forceinline__ void cluster_begun() { asm volatile("barrier.cluster.arrive.relaxed;"); }
+__device__ __forceinline__ void cluster_all_begun() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
 // Launch with the library's attributes; cluster_z > 1 asks for a thread-block
 // cluster of (1, 1, cluster_z).
 template <typename... KArgs, typename... Args>
