@@ -242,6 +242,7 @@ __device__ __forceinline__ void head_epilogue(float* recv, float* rot, uint32_t 
             }
         }
     }
+    if (ksplit > 1) rfx::cluster_all_begun();
     if (have && !mbar_wait(tmem_full_bar, 0)) {
         if (lane == 0) atomicExch(err, 3);
         have = false;
@@ -364,6 +365,8 @@ gemm_wt_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_d = tmem_base_smem;
+    // (met before anything is sent: every rank of the cluster has begun)
+    if (ksplit > 1) rfx::cluster_begun();
 
     // Let the next kernel's CTAs start as soon as every CTA of this one runs.
     rfx::pdl_launch_dependents();
@@ -515,6 +518,7 @@ gemm_wt_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         for (int pass = 0; pass < 2; ++pass) {
             const bool dry = pass == 0;
             if (!dry) {
+                if (ksplit > 1) rfx::cluster_all_begun();
                 if (have && !mbar_wait(&tmem_full_bar, 0)) {
                     if (lane == 0) atomicExch(err, 3);
                     have = false;
@@ -786,6 +790,7 @@ gemm_wt_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     // the producer and the MMA warp take part in the cluster's barrier too
     if (warp < 2 && ksplit > 1) {
         rfx::pdl_wait();
+        rfx::cluster_all_begun();
         cg::this_cluster().sync();
     }
 
