@@ -133,7 +133,8 @@ class Model:
     def load_adapters(self, folders: Mapping[str, str]) -> None:
         """Low-rank adapters by name, each from a folder (`weights.adapters`), in place of
         those loaded before.  They stay beside the weights; prompts of one `generate`
-        call may each go through another (its `adapters`)."""
+        call may each go through another (its `adapters`).  `forward_prompt`, `system1_evaluate` and the C interface go
+        without."""
         from .weights.adapters import read_adapter
 
         read = [read_adapter(folder, self.spec) for folder in folders.values()]

@@ -5,14 +5,16 @@
 //    of one adapter meet, decoding rows by the hundred) are brought by four warps with 16-byte asynchronous copies
 //    straight into the operand's swizzled layout.  K goes in up to eight pieces while that fills the GPU, a tile's
 //    pieces are a cluster, and their sums meet in distributed shared memory, in order.  v goes to memory in
-//    three bfloat16 parts (24 bits; large ranks of a bfloat16 result: two, see splits_of).  x is read once, A once a tile from the L2 cache.  8,192 rows by 4,096, three parts of rank 64: 30 to
-//    36 us where x alone would take 10; 2,047 rows by 12,288, rank 32: 25 us (x alone: 8).  What a block does once
+//    three bfloat16 parts (24 bits; large ranks of a bfloat16 result: two, see splits_of).  x is read once, A once a tile from the L2 cache.  8,192 rows by 4,096, three parts of rank 64: 30 us
+//    where x alone would take 10; 2,047 rows by 12,288, rank 32: 17 us where prompts fill their tiles, 25 where they do
+//    not (x alone: 8).  What a block does once
 //    bounds it, the barriers, the pieces' meeting and the parts' stores, beside A's way out of the cache.
 //  * up: out = base + scale B v, 128 rows by up to 4,096 of one part's columns.  v comes by TMA as the operand that it
 //    is, B's columns follow by asynchronous copies, the products go to one of two accumulators in tensor
 //    memory, and sixteen warps add them to base's rows, of which several groups of columns are always on their way.
-//    Base and out move in whole sectors, once: memory bounds it (8,192 rows by 6,144 columns, 201 MB: 51 us, 3.9 TB/s,
-//    the first and the last columns of a block included, when it only reads or only writes).
+//    Base and out move in whole sectors, once: memory bounds it (8,192 rows by 6,144 columns: 53 us in bfloat16, 201 MB,
+//    105 us in 32 bits, 403 MB: 3.8 TB/s, the first and the last columns of a block included, when it only reads or only
+//    writes).
 #include <cooperative_groups.h>
 
 #include "adapters.cuh"
@@ -288,7 +290,7 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
 // both).  Warps 0 to 15 make the sums, 32 rows by every fourth 32 columns each; warp 16 issues the products, 17 and 18
 // bring B.  AHEAD groups of base a warp are on their way or in use, 128 KB where there is room: an SM that reads
 // and writes at its share of the memory's rate waits 3 to 4 us for a load, and with 64 KB on their way (two blocks
-// of four such warps) the kernel took 58 us where it now takes 51 us for 8,192 rows by 6,144 columns.  B's
+// of four such warps) the kernel took 58 us where one of sixteen took 51 us for 8,192 rows by 6,144 columns (with v in two parts).  B's
 // columns lie in the operand, and so in tensor memory, in an order that leaves a lane of the accumulator layout
 // with eight neighbours of a row: of a group of 32, column 4 n + j is number 8 j + n (woven: even j in the first
 // half of the turn's columns, odd j in the second, each half a product with its own part of v).

@@ -15,7 +15,9 @@
 // A deeper ring is slower (four batches: 20 us): at 64 rows the memory is busy as it is, and the adapters of small
 // rank then take more of it from those of large rank, which end last.
 //
-// The low-rank rows are kept in 32 bits and go into the second product as three bfloat16 parts (24 bits).
+// The low-rank rows are kept in 32 bits and go into the second product as three bfloat16 parts (24 bits).  What the tensor
+// cores cut off is kept small: sums over K in chains of a batch, added in 32 bits, and the smallest part first (one
+// row with a 32-bit result is off by 1.3e-7; 4.4e-7 in chains of a whole slice).
 // How K is cut depends on K alone, and a row's sums on nothing else in the tile, so a row has the same bits
 // whatever shares its step.
 #include <cooperative_groups.h>

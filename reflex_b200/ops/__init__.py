@@ -420,7 +420,11 @@ def linear_geglu(x: torch.Tensor, weight_pairs: torch.Tensor) -> torch.Tensor:
 
 # ------------------------------------------------------------------ adapters
 ADAPTER_STEP_TILES = 65535  # that the launch for tiles of 16 takes; beyond, the products go by multiply-adds
-ADAPTER_STEP_ROWS = 256  # up to here rows go by tiles of 16, as requests that bring a token each; beyond by tiles of 128
+# Up to so many rows go by tiles of 16, as requests that bring a token each; beyond by tiles of 128.  The adapters of a layer's
+# four products (4,096 wide, q | k | v, o, gate and up, down) by 16 / by 128, us: 256 rows of one prompt 56 / 69 (rank
+# 16) and 92 / 83 (64), 512 rows 80 / 82 and 118 / 96, 1,024 rows 159 / 106 and 237 / 125; 256 requests over 32 adapters
+# 63 / 222 and 107 / 234.
+ADAPTER_STEP_ROWS = 256
 
 
 class AdapterRows:
@@ -507,8 +511,9 @@ class AdapterBank:
     c of x's row.  `cols`: the columns of each part of a stacked projection (q | k | v), which sum to N, each part
     with rows of `a` of its own; `woven`: two equal parts column by column (gate_0, up_0, gate_1, ...).  `ranks`
     int32 [n]: adapters of a smaller rank, whose rows of `a` and columns of `b` beyond it are zero (and are not
-    read where that saves time).  Ranks and widths that the tensor-core kernels do not take as they are (no
-    multiple of 16, of 8) are padded with zeros here, once."""
+    read where that saves time).  Beside bfloat16 a rank that is no multiple of 16 is padded with zeros here, once, for
+    the tensor-core kernels; a width that is no multiple of 8 goes by the multiply-adds, and A's rows are padded so
+    that they lie on 16 bytes."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, cols, woven: bool = False,
                  ranks: Optional[torch.Tensor] = None):

@@ -59,7 +59,9 @@ class Sampler:
     """One generation call's chooser: greedy argmax, or temperature / top-k /
     top-p with counter-based uniforms keyed by (seed, request, step).  `params` may
     be a list, one for each request of the call: every request then has its own
-    rules (and min-p), whatever shares its batch."""
+    rules (and min-p), whatever shares its batch.  Rows of a list (and min-p) go through `ops.sample_rows`, whose
+    masses are good to 2e-9, one rule for all through `ops.sample`, whose are 32-bit exponentials: from the same seed
+    about one draw in ten thousand of a flat distribution lands on the other side of a border between two tokens."""
 
     def __init__(self, params: Union[SamplingParams, Sequence[SamplingParams]], device):
         every = [params] if isinstance(params, SamplingParams) else list(params)
