@@ -15,6 +15,7 @@ import torch
 from ..errors import CudaError, InvalidInput
 import contextlib as _contextlib
 import os as _os
+import threading as _threading
 
 from . import native, workspace
 from .workspace import new as _new
@@ -487,22 +488,25 @@ def adapter_rows(ids: torch.Tensor, n: int, tile: Optional[int] = None) -> Adapt
     return rows
 
 
-_ADAPTERS: Optional[AdapterRows] = None
+class _Now(_threading.local):
+    adapters: Optional[AdapterRows] = None  # (a thread's own: another's step may run beside this one)
+
+
+_NOW = _Now()
 
 
 @_contextlib.contextmanager
 def use_adapters(rows: Optional[AdapterRows]):
     """The rows' adapters that the parts of a model go by inside the block (None: no row has one)."""
-    global _ADAPTERS
-    prev, _ADAPTERS = _ADAPTERS, rows
+    prev, _NOW.adapters = _NOW.adapters, rows
     try:
         yield rows
     finally:
-        _ADAPTERS = prev
+        _NOW.adapters = prev
 
 
 def active_adapters() -> Optional[AdapterRows]:
-    return _ADAPTERS
+    return _NOW.adapters
 
 
 class AdapterBank:
