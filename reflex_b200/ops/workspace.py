@@ -23,6 +23,7 @@ under a replay.
 from __future__ import annotations
 
 import contextlib
+import threading
 from typing import Dict, List, Optional
 
 import torch
@@ -116,36 +117,38 @@ class Workspace:
         return sum(0 if b is None else b.numel() for b in self.buffers())
 
 
-_ACTIVE: Optional[Workspace] = None
+class _Now(threading.local):
+    ws: Optional[Workspace] = None  # (a thread's own: another's step may run beside this one)
+
+
+_NOW = _Now()
 
 
 @contextlib.contextmanager
 def use(ws: Optional[Workspace]):
     """Results of `ops` calls inside the block come from `ws`."""
-    global _ACTIVE
-    prev = _ACTIVE
-    _ACTIVE = ws
+    prev, _NOW.ws = _NOW.ws, ws
     if ws is not None:
         ws.begin_step()
     try:
         yield ws
     finally:
-        _ACTIVE = prev
+        _NOW.ws = prev
 
 
 def active() -> Optional[Workspace]:
-    return _ACTIVE
+    return _NOW.ws
 
 
 def next_phase() -> None:
-    if _ACTIVE is not None:
-        _ACTIVE.next_phase()
+    if _NOW.ws is not None:
+        _NOW.ws.next_phase()
 
 
 def new(shape, dtype, device, keep: bool = False, own: bool = False) -> torch.Tensor:
     """Uninitialised memory for a result.  `keep`: lives for the whole step.
     `own`: memory of its own that outlives the step (what a step returns)."""
-    ws = _ACTIVE
+    ws = _NOW.ws
     if own or ws is None or ws.device != torch.device(device):
         return torch.empty(shape, dtype=dtype, device=device)
     return ws.take(shape, dtype, keep=keep)
@@ -153,4 +156,4 @@ def new(shape, dtype, device, keep: bool = False, own: bool = False) -> torch.Te
 
 def new_like(t: torch.Tensor) -> torch.Tensor:
     """`new` for a result of a contiguous tensor's shape and type, beside it (outside a step a little cheaper)."""
-    return torch.empty_like(t) if _ACTIVE is None else new(t.shape, t.dtype, t.device)
+    return torch.empty_like(t) if _NOW.ws is None else new(t.shape, t.dtype, t.device)

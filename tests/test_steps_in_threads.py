@@ -44,3 +44,11 @@ def test_a_thread_begins_without_adapters():
         t.start()
         t.join()
     assert seen == [None]
+
+
+def test_each_steps_working_memory():
+    from reflex_b200.ops import workspace
+
+    spaces = {who: workspace.Workspace("cpu") for who in ("mine", "other")}
+    got = beside(lambda who: workspace.use(spaces[who]), workspace.active)
+    assert got == spaces
