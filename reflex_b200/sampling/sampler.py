@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import os
 import sys
+import threading
 from typing import List, Optional, Sequence, Union
 
 import numpy as np
@@ -14,9 +15,15 @@ from .params import SamplingParams, fresh_seed, uniform
 
 
 # Pick buffers (device ids, scratch, pinned host ids, event) by (device, batch
-# size), kept for the life of the process: pinned allocations take milliseconds
-# and synchronise the device, far too much for every generation call.
-_RINGS: dict = {}
+# size), kept for the life of the thread: pinned allocations take milliseconds
+# and synchronise the device, far too much for every generation call.  (Another
+# thread's generation may run beside this one, and its picks take turns of their own.)
+class _Rings(threading.local):
+    def __init__(self):
+        self.by_size: dict = {}
+
+
+_RINGS = _Rings()
 
 
 # `REFLEX_TOP2_TRACE=1`: a numerics probe that prints, to stderr, the two
@@ -95,7 +102,7 @@ class Sampler:
     def _slot(self, n: int):
         """(ids on the device, argmax scratch, pinned host ids, event, pinned error word) for the
         next pick of n rows, from a small ring per batch size."""
-        ring = _RINGS.setdefault((str(self.device), n), {"next": 0, "slots": [None] * self.RING})
+        ring = _RINGS.by_size.setdefault((str(self.device), n), {"next": 0, "slots": [None] * self.RING})
         i = ring["next"]
         ring["next"] = (i + 1) % self.RING
         if ring["slots"][i] is None:

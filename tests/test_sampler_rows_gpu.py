@@ -1,6 +1,8 @@
 """A list of sampling parameters: what a greedy request's other parameters hold is of no account, as it is in one rule for
 all."""
 
+import threading
+
 import pytest
 import torch
 
@@ -27,3 +29,21 @@ def test_what_is_more_than_the_vocabulary_keeps_all():
     rules = [SamplingParams(temperature=1.0, seed=s, top_k=1 << 40) for s in range(3)]
     none = [SamplingParams(temperature=1.0, seed=s) for s in range(3)]
     assert Sampler(rules, DEV).pick(logits, [0, 1, 2], [0, 1, 2]) == Sampler(none, DEV).pick(logits, [0, 1, 2], [0, 1, 2])
+
+
+def test_picks_of_two_threads_take_turns_of_their_own():
+    """As many picks as a ring has, of another thread, between a pick and the reading of its ids."""
+    logits = torch.zeros(2, 500, device=DEV)
+    logits[:, 7] = 1.0
+    other = torch.zeros(2, 500, device=DEV)
+    other[:, 11] = 1.0
+    pending = Sampler(SamplingParams(), DEV).pick_async(logits, [0, 1], [0, 0])
+
+    def picks():
+        for _ in range(Sampler.RING):
+            assert Sampler(SamplingParams(), DEV).pick(other, [0, 1], [0, 0]) == [11, 11]
+
+    t = threading.Thread(target=picks)
+    t.start()
+    t.join()
+    assert pending.wait() == [7, 7] and pending.dev.tolist() == [7, 7]
