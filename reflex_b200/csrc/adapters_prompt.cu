@@ -5,9 +5,9 @@
 //    of one adapter meet, decoding rows by the hundred) are brought by four warps with 16-byte asynchronous copies
 //    straight into the operand's swizzled layout.  K goes in up to eight pieces while that fills the GPU, a tile's
 //    pieces are a cluster, and their sums meet in distributed shared memory, in order.  v goes to memory in
-//    three bfloat16 parts (24 bits; large ranks of a bfloat16 result: two, see splits_of).  x is read once, A once a tile from the L2 cache.  8,192 rows by 4,096, three parts of rank 64: 30 us
-//    where x alone would take 10; 2,047 rows by 12,288, rank 32: 17 us where prompts fill their tiles, 25 where they do
-//    not (x alone: 8).  What a block does once
+//    three bfloat16 parts (24 bits; large ranks of a bfloat16 result: two, see splits_of).  x is read once, A once a tile
+//    from the L2 cache.  8,192 rows by 4,096, three parts of rank 64: 30 us where x alone would take 10; 2,047 rows by
+//    12,288, rank 32: 17 us where prompts fill their tiles, 25 where they do not (x alone: 8).  What a block does once
 //    bounds it, the barriers, the pieces' meeting and the parts' stores, beside A's way out of the cache.
 //  * up: out = base + scale B v, 128 rows by up to 4,096 of one part's columns.  v comes by TMA as the operand that it
 //    is, B's columns follow by asynchronous copies, the products go to one of two accumulators in tensor
@@ -290,8 +290,8 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
 // both).  Warps 0 to 15 make the sums, 32 rows by every fourth 32 columns each; warp 16 issues the products, 17 and 18
 // bring B.  AHEAD groups of base a warp are on their way or in use, 128 KB where there is room: an SM that reads
 // and writes at its share of the memory's rate waits 3 to 4 us for a load, and with 64 KB on their way (two blocks
-// of four such warps) the kernel took 58 us where one of sixteen took 51 us for 8,192 rows by 6,144 columns (with v in two parts).  B's
-// columns lie in the operand, and so in tensor memory, in an order that leaves a lane of the accumulator layout
+// of four such warps) the kernel took 58 us where one of sixteen took 51 us for 8,192 rows by 6,144 columns (v in two
+// parts).  B's columns lie in the operand, and so in tensor memory, in an order that leaves a lane of the accumulator layout
 // with eight neighbours of a row: of a group of 32, column 4 n + j is number 8 j + n (woven: even j in the first
 // half of the turn's columns, odd j in the second, each half a product with its own part of v).
 template <typename TO, int SPLITS, bool WOVEN, int AHEAD>
@@ -564,8 +564,9 @@ int pieces_of(int K, int subs, int max_tiles) {
 // them B and base's groups find room for eight of a bfloat16 result, six of a 32-bit one.
 constexpr size_t MOST_SMEM = 226 * 1024;
 int v_blocks(const Args& p, int splits) { return splits * (p.parts.woven ? 2 : 1) * ((p.rank + BK - 1) / BK); }
-// The parts in which v goes from one product to the other: three (24 bits) wherever they find room, ranks to 128 (woven: to
-// 64); a bfloat16 result of larger ranks has two (16 bits: v is off by 2^-17 of itself at most, 2^-9 of the result's own rounding).
+// The parts in which v goes from one product to the other: three (24 bits) wherever they find room, ranks to 128 (woven:
+// to 64); a bfloat16 result of larger ranks has two (16 bits: v is off by 2^-17 of itself at most, 2^-9 of the result's
+// own rounding).
 int splits_of(const Args& p, int dt_out) { return dt_out == RFX_DT_F32 || v_blocks(p, 3) <= 6 ? 3 : 2; }
 
 template <typename TO, int SPLITS, bool WOVEN>

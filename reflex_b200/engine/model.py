@@ -143,7 +143,8 @@ class CausalLM:
 
     def bind_adapters(self, adapters, names=()) -> None:
         """`adapters`: what `weights.adapters.read_adapter` gave for each, and their names where they have any; they
-        take the place of those bound before (`Engine.load_adapters` sees to the engines that run the model).  Nothing changes where one of them names a matrix that its part does not take adapters for."""
+        take the place of those bound before (`Engine.load_adapters` sees to the engines that run the model).  Nothing
+        changes where one of them names a matrix that its part does not take adapters for."""
         exp = expected_tensors(self.spec)
         parts: Dict[Tuple[int, str], Dict[str, list]] = {}
         for i, adapter in enumerate(adapters):
